@@ -1,0 +1,114 @@
+/*
+ * vt_micro_abi.h -- C ABI of the ray-head operators of libvt_hip.so: numbers
+ * in microscaled formats (4 bits for serving, 8 bits for what a training step
+ * keeps) and the products that read them.  The conventions are those of
+ * vt_abi.h: device pointers, a hipStream_t, 0 or a VT_ERR_* code,
+ * vt_last_error() for the message, no synchronisation, workspaces owned by
+ * the caller.  These operators have no counterpart in the reference.
+ *
+ * Formats.  A row is divided into blocks of 32 consecutive values, the last
+ * one shorter where the width is no multiple of 32.  A block's scale is an
+ * e8m0 byte c, the power of two 2^(c - 127); 255 is NaN.
+ *   mx4: e2m1 codes (0, 1/2, 1, 3/2, 2, 3, 4, 6 and their negatives, the sign
+ *     in bit 3), two a byte, the even position in the low nibble.  codes u8
+ *     (rows, 16 * blocks), the positions past the width zero; scales u8
+ *     (rows, blocks).  A scale is 2^(floor(log2 max|x|) - 2), at least 2^-127;
+ *     values are rounded to nearest even and held to 6.  A block that holds a
+ *     NaN or an infinity has scale 255 and reads as NaN.
+ *   ckpt8: e4m3 codes (bias 7, no infinities, 0x7f NaN), one a byte.  codes
+ *     u8 (rows, width); scales u8 (rows, blocks).  A scale is
+ *     2^(floor(log2 m) - 7) for the largest finite magnitude m, at least
+ *     2^-127, so that nothing is held back; values are rounded to nearest
+ *     even, except that only zeros become zero (a magnitude below half of the
+ *     smallest, 2^-9 of the scale, becomes it): the slope of ReLU is that of
+ *     the value itself.  A NaN or an infinity is kept as NaN, alone.
+ */
+#ifndef VT_MICRO_ABI_H
+#define VT_MICRO_ABI_H
+
+#include "vt_abi.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* Element types of x, y, z, dy and dz.  VT_MX4 (vt_mx4_linear's x only): rows
+ * that are stored in 4 bits already. */
+enum { VT_F32 = 0, VT_F16 = 1, VT_BF16 = 2, VT_MX4 = 3 };
+/* Activations: z, max(z, 0), z / (1 + exp(-z)), z (1 + erf(z / sqrt 2)) / 2. */
+enum { VT_ACT_NONE = 0, VT_ACT_RELU = 1, VT_ACT_SILU = 2, VT_ACT_GELU = 3 };
+
+/* x (rows, width) of `dtype`, rows x_stride elements apart -> codes, scales. */
+int vt_mx4_quantize(int dtype, const void *x, int64_t x_stride, uint64_t rows, uint32_t width, uint8_t *codes,
+                    uint8_t *scales, vt_stream_t stream);
+/* codes, scales -> out (rows, width) of `dtype`, contiguous; each value is
+ * rounded once to the type. */
+int vt_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, uint64_t rows, uint32_t width, int dtype, void *out,
+                      vt_stream_t stream);
+
+/*
+ * y[m][n] = sum_k xq[m][k] wq[n][k] + bias[n], with relu max(y, 0): the
+ * product of x's rows in 4 bits with weights in 4 bits (out rows of `width`).
+ * x of VT_F32, VT_F16 or VT_BF16 (rows x_stride elements apart, x_scales
+ * unused) is quantised on the way by vt_mx4_quantize's rule; VT_MX4 takes
+ * codes and x_scales, contiguous.  Sums are f32, rounded once to y_dtype.
+ * bias: f32 (out) or NULL.  y (rows, out), contiguous.  width 0 gives the
+ * bias.  workspace: vt_mx4_linear_workspace_size bytes, 16-byte aligned.
+ */
+size_t vt_mx4_linear_workspace_size(int x_dtype, uint64_t rows, uint32_t width, uint32_t out);
+int vt_mx4_linear(int x_dtype, const void *x, int64_t x_stride, const uint8_t *x_scales, uint64_t rows, uint32_t width,
+                  const uint8_t *w_codes, const uint8_t *w_scales, uint32_t out, const float *bias, int relu,
+                  int y_dtype, void *y, void *workspace, vt_stream_t stream);
+
+/* One layer of vt_mx4_mlp: weights mx4 (out, width), bias f32 (out) or NULL. */
+typedef struct vt_mx4_layer {
+    const uint8_t *codes;
+    const uint8_t *scales;
+    const float *bias;
+    uint32_t width;
+    uint32_t out;
+} vt_mx4_layer;
+
+/*
+ * A whole head: layers in turn, each as vt_mx4_linear, ReLU behind all but
+ * the last; hidden values go from f32 to 4 bits without another rounding.
+ * layers: host array; layers[i].width == layers[i - 1].out.  x as above (not
+ * VT_MX4), y (rows, layers[last].out) of y_dtype, contiguous.
+ */
+enum { VT_MX4_MAX_LAYERS = 16 };
+size_t vt_mx4_mlp_workspace_size(int x_dtype, uint64_t rows, const vt_mx4_layer *layers, uint32_t num_layers);
+int vt_mx4_mlp(int x_dtype, const void *x, int64_t x_stride, uint64_t rows, const vt_mx4_layer *layers,
+               uint32_t num_layers, int y_dtype, void *y, void *workspace, vt_stream_t stream);
+
+/*
+ * An activation that keeps its input: z (rows, width) of `dtype`, rows
+ * z_stride elements apart -> y = act(z) of `dtype`, contiguous, from z itself
+ * (NULL with VT_ACT_NONE: not written), and z's ckpt8 codes and scales.
+ */
+int vt_act_checkpoint(int dtype, int act, const void *z, int64_t z_stride, uint64_t rows, uint32_t width, void *y,
+                      uint8_t *codes, uint8_t *scales, vt_stream_t stream);
+/* codes, scales -> out (rows, width) of `dtype`, contiguous. */
+int vt_ckpt8_dequantize(const uint8_t *codes, const uint8_t *scales, uint64_t rows, uint32_t width, int dtype,
+                        void *out, vt_stream_t stream);
+/* dz = dy act'(z^), z^ the values the checkpoint holds; dy and dz of `dtype`,
+ * dy's rows dy_stride elements apart, dz contiguous.  ReLU's slope at 0 is 0;
+ * where z^ is NaN so is dz. */
+int vt_act_input_grad(int dtype, int act, const uint8_t *codes, const uint8_t *scales, const void *dy,
+                      int64_t dy_stride, uint64_t rows, uint32_t width, void *dz, vt_stream_t stream);
+/*
+ * Gradients of a layer y = act(z) W^T + b behind the activation, from the
+ * checkpoint of z: dw[n][k] = sum_m dy[m][n] act(z^)[m][k], f32 (out, width),
+ * and, where db is not NULL, db[n] = sum_m dy[m][n], f32 (out).  dy (rows,
+ * out) of `dtype`, rows dy_stride elements apart.  Sums are f32 in a fixed
+ * order (the same inputs give the same bits).  workspace:
+ * vt_act_weight_grad_workspace_size bytes, 16-byte aligned.
+ */
+size_t vt_act_weight_grad_workspace_size(uint64_t rows, uint32_t width, uint32_t out);
+int vt_act_weight_grad(int dtype, int act, const uint8_t *codes, const uint8_t *scales, const void *dy,
+                       int64_t dy_stride, uint64_t rows, uint32_t width, uint32_t out, float *dw, float *db,
+                       void *workspace, vt_stream_t stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif

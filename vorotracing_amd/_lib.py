@@ -17,8 +17,10 @@ P = C.c_void_p
 U32 = C.c_uint32
 F32 = C.c_float
 I32 = C.c_int
+I64 = C.c_int64
+U64 = C.c_uint64
 
-# name -> argtypes (restype int unless noted); mirrors include/vt_abi.h
+# name -> argtypes (restype int unless noted); mirrors include/vt_abi.h and include/vt_micro_abi.h
 SIGNATURES = {
     "vt_last_error": ([], C.c_char_p),
     "vt_abi_version": ([], C.c_int),
@@ -84,6 +86,18 @@ SIGNATURES = {
     "vt_quantize_u8": ([P, U32, U32, I32, P, P, P, P], C.c_int),
     "vt_quantize_workspace_size": ([], C.c_size_t),
     "vt_pad_3to4_f16": ([P, U32, U32, P, P], C.c_int),
+    # include/vt_micro_abi.h
+    "vt_mx4_quantize": ([I32, P, I64, U64, U32, P, P, P], C.c_int),
+    "vt_mx4_dequantize": ([P, P, U64, U32, I32, P, P], C.c_int),
+    "vt_mx4_linear_workspace_size": ([I32, U64, U32, U32], C.c_size_t),
+    "vt_mx4_linear": ([I32, P, I64, P, U64, U32, P, P, U32, P, I32, I32, P, P, P], C.c_int),
+    "vt_mx4_mlp_workspace_size": ([I32, U64, P, U32], C.c_size_t),
+    "vt_mx4_mlp": ([I32, P, I64, U64, P, U32, I32, P, P, P], C.c_int),
+    "vt_act_checkpoint": ([I32, I32, P, I64, U64, U32, P, P, P, P], C.c_int),
+    "vt_ckpt8_dequantize": ([P, P, U64, U32, I32, P, P], C.c_int),
+    "vt_act_input_grad": ([I32, I32, P, P, P, I64, U64, U32, P, P], C.c_int),
+    "vt_act_weight_grad_workspace_size": ([U64, U32, U32], C.c_size_t),
+    "vt_act_weight_grad": ([I32, I32, P, P, P, I64, U64, U32, U32, P, P, P, P], C.c_int),
 }
 
 

@@ -1,0 +1,144 @@
+// vt_micro.h -- device code shared by the ray-head operators: element types,
+// block scales, 4- and 8-bit conversions (formats: include/vt_micro_abi.h).
+#pragma once
+
+#include "vt_internal.h"
+
+#include "../../include/vt_micro_abi.h"
+
+namespace vt {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// global rows start at any multiple of their element: gfx950 takes vector
+// loads and stores at such addresses
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
+
+constexpr uint32_t MX_BLOCK = 32; // values under one scale
+constexpr uint32_t MX_NAN = 255;  // the scale of a block that reads as NaN
+
+inline __host__ __device__ uint32_t mx_blocks(uint32_t width) { return (width + MX_BLOCK - 1) / MX_BLOCK; }
+
+// 2^(c - 127); c = 0 is the subnormal 2^-127, 255 NaN
+__device__ __forceinline__ float e8m0_value(uint32_t c)
+{
+    const uint32_t bits = c == 0 ? 0x00400000u : c == MX_NAN ? 0x7fc00000u : c << 23;
+    return __builtin_bit_cast(float, bits);
+}
+
+// 2^(127 - c) for c <= 254
+__device__ __forceinline__ float e8m0_inverse(uint32_t c) { return e8m0_value(254 - c); }
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
+
+// Scale byte of an mx4 block from the largest magnitude's bits (compared as
+// integers, so that NaN and infinity come out on top).
+__device__ __forceinline__ uint32_t mx4_scale(uint32_t top)
+{
+    const uint32_t e = top >> 23;
+    return e == 255 ? MX_NAN : e > 2 ? e - 2 : 0;
+}
+
+// Two values over 1 to e2m1, in the low byte: nearest even, held to 6.
+__device__ __forceinline__ uint32_t e2m1_pair(float a, float b)
+{
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, a, b, 1.0f, 0);
+}
+
+// ---- element types: eight consecutive values at a time
+
+template <typename T>
+struct Elem;
+template <>
+struct Elem<float> {
+    static constexpr int code = VT_F32;
+    static __device__ __forceinline__ void load8(const float *p, float v[8])
+    {
+        const u32x4 a = *reinterpret_cast<const u32x4_any *>(p), b = *reinterpret_cast<const u32x4_any *>(p + 4);
+        for (int i = 0; i < 4; ++i) {
+            v[i] = __builtin_bit_cast(float, (uint32_t)a[i]);
+            v[4 + i] = __builtin_bit_cast(float, (uint32_t)b[i]);
+        }
+    }
+    static __device__ __forceinline__ void store8(float *p, const float v[8])
+    {
+        u32x4 a, b;
+        for (int i = 0; i < 4; ++i) {
+            a[i] = __builtin_bit_cast(uint32_t, v[i]);
+            b[i] = __builtin_bit_cast(uint32_t, v[4 + i]);
+        }
+        *reinterpret_cast<u32x4_any *>(p) = a;
+        *reinterpret_cast<u32x4_any *>(p + 4) = b;
+    }
+};
+template <typename T>
+struct Elem16 {
+    static __device__ __forceinline__ void load8(const T *p, float v[8])
+    {
+        typedef T t8 __attribute__((ext_vector_type(8)));
+        const t8 h = __builtin_bit_cast(t8, (u32x4) * reinterpret_cast<const u32x4_any *>(p));
+        for (int i = 0; i < 8; ++i)
+            v[i] = (float)h[i];
+    }
+    static __device__ __forceinline__ void store8(T *p, const float v[8])
+    {
+        typedef T t8 __attribute__((ext_vector_type(8)));
+        t8 h;
+        for (int i = 0; i < 8; ++i)
+            h[i] = (T)v[i];
+        *reinterpret_cast<u32x4_any *>(p) = __builtin_bit_cast(u32x4, h);
+    }
+};
+template <>
+struct Elem<_Float16> : Elem16<_Float16> {
+    static constexpr int code = VT_F16;
+};
+template <>
+struct Elem<__bf16> : Elem16<__bf16> {
+    static constexpr int code = VT_BF16;
+};
+
+// v[0..8) = p[0..n), zeros behind (n <= 8)
+template <typename T>
+__device__ __forceinline__ void load_upto8(const T *p, uint32_t n, float v[8])
+{
+    if (n >= 8) {
+        Elem<T>::load8(p, v);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+            v[i] = i < n ? (float)p[i] : 0.0f;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_upto8(T *p, uint32_t n, const float v[8])
+{
+    if (n >= 8) {
+        Elem<T>::store8(p, v);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+            if (i < n)
+                p[i] = (T)v[i];
+    }
+}
+
+// Host: run a generic lambda with the element type of `dtype`.
+template <typename F>
+inline int with_type(int dtype, F &&f)
+{
+    switch (dtype) {
+    case VT_F32: return f(float());
+    case VT_F16: return f(_Float16());
+    case VT_BF16: return f(__bf16());
+    }
+    set_error("dtype %d is none of VT_F32, VT_F16, VT_BF16", dtype);
+    return VT_ERR_INVALID;
+}
+
+} // namespace vt

@@ -1,0 +1,327 @@
+"""Operators behind the tracer in microscaled formats (include/vt_micro_abi.h):
+numbers in blocks of 32 under one power of two, held in 4 bits where a scene is
+served and in 8 where a training step keeps an activation for its backward
+pass.  No counterpart in the reference.
+
+Serving:
+
+* ``quantize_mx4(x)`` puts rows into 4 bits (``Mx4``); ``Mx4.dequantize``
+  reads them;
+* ``linear_mx4(x, weight, bias)`` multiplies rows, quantised on the way or
+  stored as ``Mx4``, with weights in 4 bits;
+* ``mlp_mx4(x, layers)`` runs a head of such layers with ReLU between them.
+
+Training:
+
+* ``checkpoint_activation(z, activation)`` gives ``act(z)`` and a
+  ``Checkpoint8`` of z, a quarter of the bytes of f32;
+* ``Checkpoint8.input_grad(dy)`` and ``Checkpoint8.weight_grad(dy)`` are what
+  the backward pass needs of it (``head.activated_linear`` is the autograd
+  function made of them).
+
+Tensors are on the GPU, float32, float16 or bfloat16, of any leading shape;
+rows may be strided, a last dimension that is not unit-stride is copied.  Work
+is enqueued on torch's current stream of the tensors' device.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import _lib, native
+
+BLOCK = 32  # values under one scale
+MAX_LAYERS = 16
+_MX4 = 3  # VT_MX4
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+
+
+def _blocks(width: int) -> int:
+    return -(-width // BLOCK)
+
+
+def _check(t: torch.Tensor, what: str) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what}: expected a tensor, got {type(t).__name__}")
+    if t.dtype not in _DTYPES:
+        raise ValueError(f"{what}: expected float32, float16 or bfloat16, got {t.dtype}")
+    if not t.is_cuda:
+        raise ValueError(f"{what}: expected a GPU tensor, got one on {t.device}")
+    if t.dim() == 0:
+        raise ValueError(f"{what}: expected rows, got a scalar")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: this operator records no gradient (head.activated_linear does); detach the tensor")
+    return t
+
+
+def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
+    """(t with unit stride along its rows, the number of rows, elements from row to row)."""
+    width = t.shape[-1]
+    if t.is_contiguous():
+        return t, t.numel() // width if width else math.prod(t.shape[:-1]), width
+    if width == 0:
+        return t, math.prod(t.shape[:-1]), 0
+    t = t.reshape(-1, width)
+    if t.stride(1) != 1 and width > 1:
+        t = t.contiguous()
+    return t, t.shape[0], t.stride(0)
+
+
+def _same_device(what: str, device, *tensors):
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: tensors on {device} and {t.device}")
+
+
+def _call(name: str, device, *args):
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            _lib.call(name, *args, native._s(device))
+    else:
+        _lib.call(name, *args, native._s(device))
+
+
+def _workspace(size: int, device) -> Optional[torch.Tensor]:
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+
+
+def _check_codes(what: str, codes, scales, lead_width: int, blocks: int):
+    for t, name, last in ((codes, "codes", lead_width), (scales, "scales", blocks)):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.uint8 or not t.is_cuda:
+            raise ValueError(f"{what}: {name} are a uint8 tensor on the GPU")
+        if t.dim() == 0 or t.shape[-1] != last:
+            raise ValueError(f"{what}: {name} have {tuple(t.shape)}, expected rows of {last}")
+        if not t.is_contiguous():
+            raise ValueError(f"{what}: {name} have to be contiguous")
+    if codes.shape[:-1] != scales.shape[:-1]:
+        raise ValueError(f"{what}: codes of {tuple(codes.shape)} with scales of {tuple(scales.shape)}")
+    _same_device(what, codes.device, scales)
+
+
+class Mx4:
+    """Rows of ``width`` values in 4 bits: ``codes`` u8 (..., 16 * blocks), two
+    e2m1 values a byte, and ``scales`` u8 (..., blocks), e8m0, for blocks of 32
+    (0.53 bytes a value).  ``quantize_mx4`` makes one; the constructor takes
+    tensors that were stored."""
+
+    __slots__ = ("codes", "scales", "width")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, width: int):
+        blocks = _blocks(width)
+        _check_codes("Mx4", codes, scales, 16 * blocks, blocks)
+        self.codes, self.scales, self.width = codes, scales, int(width)
+
+    @property
+    def shape(self) -> torch.Size:
+        return torch.Size((*self.codes.shape[:-1], self.width))
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def rows(self) -> int:
+        return math.prod(self.codes.shape[:-1])
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values, rounded once to ``dtype``."""
+        if dtype not in _DTYPES:
+            raise ValueError(f"dequantize: expected float32, float16 or bfloat16, got {dtype}")
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        _call("vt_mx4_dequantize", self.device, self.codes.data_ptr(), self.scales.data_ptr(), self.rows, self.width,
+              _DTYPES[dtype], out.data_ptr())
+        return out
+
+    def __repr__(self):
+        return f"Mx4(shape={tuple(self.shape)}, device={self.device})"
+
+
+def quantize_mx4(x: torch.Tensor) -> Mx4:
+    """Rows of x in 4 bits, in blocks of 32 along the last dimension: a block's
+    scale is 2^(floor(log2 max|x|) - 2), its values are rounded to nearest even
+    among 0, 1/2, 1, 3/2, 2, 3, 4, 6 of it (larger quotients, below 8, become
+    6).  A block with a NaN or an infinity reads as NaN."""
+    _check(x, "quantize_mx4")
+    lead, width = x.shape[:-1], x.shape[-1]
+    blocks = _blocks(width)
+    codes = torch.empty((*lead, 16 * blocks), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((*lead, blocks), dtype=torch.uint8, device=x.device)
+    x, rows, stride = _rows(x)
+    _call("vt_mx4_quantize", x.device, _DTYPES[x.dtype], x.data_ptr(), stride, rows, width, codes.data_ptr(),
+          scales.data_ptr())
+    return Mx4(codes, scales, width)
+
+
+def _check_layer(what: str, weight, bias, width: int, device):
+    if not isinstance(weight, Mx4) or weight.codes.dim() != 2:
+        raise ValueError(f"{what}: weights are an Mx4 of (out, width)")
+    if weight.width != width:
+        raise ValueError(f"{what}: rows of {width} values with weights of {tuple(weight.shape)}")
+    if bias is not None:
+        if bias.dtype != torch.float32 or tuple(bias.shape) != (weight.codes.shape[0],) or not bias.is_contiguous():
+            raise ValueError(f"{what}: the bias is a contiguous float32 tensor of {weight.codes.shape[0]}")
+    _same_device(what, device, weight.codes, bias)
+
+
+def _out_dtype(what: str, dtype, default):
+    dtype = default if dtype is None else dtype
+    if dtype not in _DTYPES:
+        raise ValueError(f"{what}: expected float32, float16 or bfloat16, got {dtype}")
+    return dtype
+
+
+def linear_mx4(x: Union[torch.Tensor, Mx4], weight: Mx4, bias: Optional[torch.Tensor] = None, *, relu: bool = False,
+               dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """x W^T + bias for weights in 4 bits, with ``relu`` its positive part: x
+    (..., width) is quantised on the way as ``quantize_mx4`` does, or is an
+    ``Mx4`` already.  Sums are float32, rounded once to ``dtype`` (x's own, or
+    float32 for an ``Mx4``).  No gradient is recorded."""
+    stored = isinstance(x, Mx4)
+    if not stored:
+        _check(x, "linear_mx4")
+    width, device, lead = x.shape[-1], x.device, x.shape[:-1]
+    _check_layer("linear_mx4", weight, bias, width, device)
+    dtype = _out_dtype("linear_mx4", dtype, torch.float32 if stored else x.dtype)
+    out = weight.codes.shape[0]
+    y = torch.empty((*lead, out), dtype=dtype, device=device)
+    if stored:
+        code, at, scales, rows, stride = _MX4, x.codes.data_ptr(), x.scales.data_ptr(), x.rows, 0
+    else:
+        code = _DTYPES[x.dtype]
+        x, rows, stride = _rows(x)
+        at, scales = x.data_ptr(), None
+    ws = _workspace(_lib.load().vt_mx4_linear_workspace_size(code, rows, width, out), device)
+    _call("vt_mx4_linear", device, code, at, stride, scales, rows, width, weight.codes.data_ptr(),
+          weight.scales.data_ptr(), out, native._p(bias), int(relu), _DTYPES[dtype], y.data_ptr(), native._p(ws))
+    return y
+
+
+class _LayerC(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("bias", C.c_void_p), ("width", C.c_uint32),
+                ("out", C.c_uint32)]
+
+
+def mlp_mx4(x: torch.Tensor, layers: Sequence[Tuple[Mx4, Optional[torch.Tensor]]], *,
+            dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """A head of ``layers`` ((weight, bias) pairs, 1 to 16) over the rows of x,
+    each as ``linear_mx4``, with ReLU behind all but the last.  Hidden values
+    go from float32 to 4 bits without another rounding; the result is rounded
+    once to ``dtype`` (x's own).  No gradient is recorded."""
+    _check(x, "mlp_mx4")
+    if not 1 <= len(layers) <= MAX_LAYERS:
+        raise ValueError(f"mlp_mx4: 1 to {MAX_LAYERS} layers, got {len(layers)}")
+    dtype = _out_dtype("mlp_mx4", dtype, x.dtype)
+    lead, width, device = x.shape[:-1], x.shape[-1], x.device
+    table = (_LayerC * len(layers))()
+    for entry, (weight, bias) in zip(table, layers):
+        _check_layer("mlp_mx4", weight, bias, width, device)
+        if width == 0 or weight.codes.shape[0] == 0:
+            raise ValueError("mlp_mx4: a layer without inputs or outputs")
+        entry.codes, entry.scales = weight.codes.data_ptr(), weight.scales.data_ptr()
+        entry.bias = native._p(bias)
+        entry.width, entry.out = width, weight.codes.shape[0]
+        width = weight.codes.shape[0]
+    y = torch.empty((*lead, width), dtype=dtype, device=device)
+    x, rows, stride = _rows(x)
+    at, code = C.addressof(table), _DTYPES[x.dtype]
+    ws = _workspace(_lib.load().vt_mx4_mlp_workspace_size(code, rows, at, len(layers)), device)
+    _call("vt_mx4_mlp", device, code, x.data_ptr(), stride, rows, at, len(layers), _DTYPES[dtype], y.data_ptr(),
+          native._p(ws))
+    return y
+
+
+class Checkpoint8:
+    """The input z of an activation in 8 bits: ``codes`` u8 (..., width), one
+    e4m3 value a byte, and ``scales`` u8 (..., blocks), e8m0, for blocks of 32
+    (1.03 bytes a value), with the activation's name.  A value differs from
+    z's by at most 2^-4 of itself, or by 2^-9 of its block's scale (2^-16 of
+    the block's largest magnitude or less) where it is far below that; zero,
+    and only zero, is kept as zero, and a NaN or an infinity as NaN.
+    ``checkpoint_activation`` makes one."""
+
+    __slots__ = ("codes", "scales", "activation")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, activation: str):
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"activation {activation!r} is none of {', '.join(ACTIVATIONS)}")
+        width = codes.shape[-1] if isinstance(codes, torch.Tensor) and codes.dim() else 0
+        _check_codes("Checkpoint8", codes, scales, width, _blocks(width))
+        self.codes, self.scales, self.activation = codes, scales, activation
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.codes.shape
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """z as the checkpoint holds it, rounded once to ``dtype``."""
+        dtype = _out_dtype("dequantize", dtype, None)
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        width = self.shape[-1]
+        _call("vt_ckpt8_dequantize", self.device, self.codes.data_ptr(), self.scales.data_ptr(),
+              math.prod(self.shape[:-1]), width, _DTYPES[dtype], out.data_ptr())
+        return out
+
+    def input_grad(self, dy: torch.Tensor) -> torch.Tensor:
+        """dz = dy act'(z^), of dy's type: the gradient behind the activation
+        brought before it.  ReLU's slope is 0 at 0; a NaN in z^ stays one."""
+        _check(dy, "input_grad")
+        if dy.shape != self.shape:
+            raise ValueError(f"input_grad: a gradient of {tuple(dy.shape)} for activations of {tuple(self.shape)}")
+        _same_device("input_grad", self.device, dy)
+        dz = torch.empty(self.shape, dtype=dy.dtype, device=self.device)
+        dy, rows, stride = _rows(dy)
+        _call("vt_act_input_grad", self.device, _DTYPES[dy.dtype], ACTIVATIONS[self.activation],
+              self.codes.data_ptr(), self.scales.data_ptr(), dy.data_ptr(), stride, rows, self.shape[-1],
+              dz.data_ptr())
+        return dz
+
+    def weight_grad(self, dy: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(dW, db) of a layer act(z) W^T + b behind the activation, for its
+        output's gradient dy (..., out): dW = dy^T act(z^) (out, width) and
+        db, dy's sum over the rows (out,), both float32.  The same inputs give
+        the same bits."""
+        _check(dy, "weight_grad")
+        if dy.shape[:-1] != self.shape[:-1]:
+            raise ValueError(f"weight_grad: a gradient of {tuple(dy.shape)} for activations of {tuple(self.shape)}")
+        _same_device("weight_grad", self.device, dy)
+        out, width = dy.shape[-1], self.shape[-1]
+        dy, rows, stride = _rows(dy)
+        dw = torch.empty((out, width), dtype=torch.float32, device=self.device)
+        db = torch.empty(out, dtype=torch.float32, device=self.device)
+        ws = _workspace(_lib.load().vt_act_weight_grad_workspace_size(rows, width, out), self.device)
+        _call("vt_act_weight_grad", self.device, _DTYPES[dy.dtype], ACTIVATIONS[self.activation],
+              self.codes.data_ptr(), self.scales.data_ptr(), dy.data_ptr(), stride, rows, width, out, dw.data_ptr(),
+              db.data_ptr(), native._p(ws))
+        return dw, db
+
+    def __repr__(self):
+        return f"Checkpoint8(shape={tuple(self.shape)}, activation={self.activation!r}, device={self.device})"
+
+
+def checkpoint_activation(z: torch.Tensor, activation: str) -> Tuple[torch.Tensor, Checkpoint8]:
+    """(act(z), the 8-bit checkpoint of z): act(z) is computed from z itself
+    and has its type; for "none" it is z.  ``activation``: "none", "relu",
+    "silu" (z / (1 + exp(-z))) or "gelu" (z (1 + erf(z / sqrt 2)) / 2).  No
+    gradient is recorded; the checkpoint's methods are the backward pass."""
+    _check(z, "checkpoint_activation")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation {activation!r} is none of {', '.join(ACTIVATIONS)}")
+    shape, width = z.shape, z.shape[-1]
+    codes = torch.empty(shape, dtype=torch.uint8, device=z.device)
+    scales = torch.empty((*shape[:-1], _blocks(width)), dtype=torch.uint8, device=z.device)
+    y = z if activation == "none" else torch.empty(shape, dtype=z.dtype, device=z.device)
+    src, rows, stride = _rows(z)
+    _call("vt_act_checkpoint", z.device, _DTYPES[z.dtype], ACTIVATIONS[activation], src.data_ptr(), stride, rows, width,
+          None if activation == "none" else y.data_ptr(), codes.data_ptr(), scales.data_ptr())
+    return y, Checkpoint8(codes, scales, activation)
+
+
+__all__ = ["Mx4", "quantize_mx4", "linear_mx4", "mlp_mx4", "Checkpoint8", "checkpoint_activation", "ACTIVATIONS"]
