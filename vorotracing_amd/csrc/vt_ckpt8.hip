@@ -158,68 +158,237 @@ __global__ __launch_bounds__(ACT_THREADS) void ckpt8_read_kernel(const uint8_t *
     store_upto8(out + row * width + k, n, v);
 }
 
-// dw[n][k] += dy[m][n] act(z^[m][k]) over one range of rows a block: a tile of
-// 16 n by 16 k, one output a thread, rows staged in shared memory.
-constexpr int WG_TILE = 16, WG_ROWS = 32;
+// ---- the gradient of the weights: dw[n][k] = sum_m dy[m][n] act(z^)[m][k]
+//
+// A product whose contraction runs over the rows, the slow axis of both
+// operands.  A block of four waves sums a tile of 128 n by 128 k over a range
+// of rows, 32 at a time: dy and act(z^) go to shared memory as bf16 rows, and
+// the transposing read (ds_read_b64_tr_b16) hands each lane the 8 rows of one
+// column that v_mfma_f32_16x16x32_bf16 wants of it.
+//
+// An e4m3 value under its scale is exact in bf16, and so is its ReLU: against
+// a bf16 gradient the product is one matrix instruction with nothing rounded
+// but the f32 sum.  A wider factor is split into bf16 parts that hold all of
+// its bits (f16: 2, f32 and the smooth activations: 3), and the products of
+// parts down to 2^-16 of the first are summed (2, 3, 5 or 6 instructions).
+constexpr int WG_THREADS = 256, WG_N = 128, WG_K = 128, WG_M = 32;
+// 288 bytes a row: the four rows of a transposing read fall into different banks
+constexpr int WG_PITCH = 144;
 
-template <typename T, int ACT>
-__global__ __launch_bounds__(WG_TILE *WG_TILE) void weight_grad_kernel(
-    const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, const T *__restrict__ dy, int64_t dy_stride,
-    uint64_t rows, uint64_t rows_per_split, uint32_t width, uint32_t out, float *__restrict__ dw, float *__restrict__ db)
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint16_t WgTile[WG_M][WG_PITCH];
+
+template <typename T>
+constexpr int dy_parts = sizeof(T) == 4 ? 3 : std::is_same<T, _Float16>::value ? 2 : 1;
+template <int ACT>
+constexpr int act_parts = ACT == VT_ACT_SILU || ACT == VT_ACT_GELU ? 3 : 1;
+
+// The first P bf16 parts of v, cut off and not rounded: three hold every bit
+// of an f32, two every bit of an f16.  What is not finite is its first part.
+template <int P>
+__device__ __forceinline__ void bf16_parts(float v, uint16_t part[P])
 {
-    __shared__ float a[WG_ROWS][WG_TILE + 1], b[WG_ROWS][WG_TILE + 1];
-    const uint32_t tk = threadIdx.x % WG_TILE, tn = threadIdx.x / WG_TILE;
-    const uint32_t k0 = blockIdx.x * WG_TILE, n0 = blockIdx.y * WG_TILE;
-    const uint64_t m1 = min(rows, (blockIdx.z + 1) * rows_per_split);
-    float sum = 0.0f, sum_b = 0.0f;
-    for (uint64_t m0 = blockIdx.z * rows_per_split; m0 < m1; m0 += WG_ROWS) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < WG_ROWS * WG_TILE; i += WG_TILE * WG_TILE) {
-            const uint32_t r = i / WG_TILE, c = i % WG_TILE;
-            const uint64_t m = m0 + r;
-            float d = 0.0f, v = 0.0f;
-            if (m < m1 && n0 + c < out)
-                d = (float)dy[(int64_t)m * dy_stride + n0 + c];
-            if (m < m1 && k0 + c < width) {
-                float q[4];
-                e4m3_values(codes[m * width + k0 + c], e8m0_value(scales[m * mx_blocks(width) + (k0 + c) / MX_BLOCK]), q);
-                v = act_value<ACT>(q[0]);
-            }
-            a[r][c] = d;
-            b[r][c] = v;
-        }
-        __syncthreads();
-        for (int r = 0; r < WG_ROWS; ++r) {
-            sum = __builtin_fmaf(a[r][tn], b[r][tk], sum);
-            sum_b += a[r][tn];
+    if constexpr (P == 1) {
+        part[0] = __builtin_bit_cast(uint16_t, (__bf16)v);
+    } else {
+        const uint32_t b = __builtin_bit_cast(uint32_t, v);
+        const bool finite = (b & 0x7f800000u) != 0x7f800000u;
+        part[0] = v != v ? 0x7fc0 : (uint16_t)(b >> 16);
+        float r = finite ? v - __builtin_bit_cast(float, b & 0xffff0000u) : 0.0f;
+#pragma unroll
+        for (int i = 1; i < P; ++i) {
+            const uint32_t rb = __builtin_bit_cast(uint32_t, r);
+            part[i] = (uint16_t)(rb >> 16);
+            r -= __builtin_bit_cast(float, rb & 0xffff0000u);
         }
     }
-    const uint32_t n = n0 + tn, k = k0 + tk;
-    if (n < out && k < width)
-        dw[((uint64_t)blockIdx.z * out + n) * width + k] = sum;
-    if (db && n < out && k == 0)
-        db[(uint64_t)blockIdx.z * out + n] = sum_b;
 }
 
-// Joins the ranges' sums in their order.
-__global__ __launch_bounds__(256) void weight_join_kernel(const float *__restrict__ parts, uint32_t splits, uint64_t n,
-                                                          float *__restrict__ to)
+// Eight values as P parts into P tiles at (row, col), col a multiple of 8.
+template <int P>
+__device__ __forceinline__ void store_parts(WgTile *tile, uint32_t row, uint32_t col, const float v[8])
 {
-    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n)
-        return;
-    float s = 0.0f;
-    for (uint32_t p = 0; p < splits; ++p)
-        s += parts[p * n + i];
-    to[i] = s;
+    uint16_t part[8][P];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        bf16_parts<P>(v[i], part[i]);
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            w[i] = part[2 * i][p] | (uint32_t)part[2 * i + 1][p] << 16;
+        *reinterpret_cast<u32x4 *>(&tile[p][row][col]) = w;
+    }
 }
 
+// A lane's operand: rows 8 g .. 8 g + 7 of column col + lane % 16.
+__device__ __forceinline__ bf16x8 read_columns(WgTile &tile, uint32_t col, uint32_t lane)
+{
+    typedef __attribute__((address_space(3))) s16x4 lds4;
+    const uint32_t i = lane & 15, row = 8 * (lane >> 4) + i / 4, at = col + 4 * (i & 3);
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)&tile[row][at]);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)&tile[row + 4][at]);
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+struct WeightArgs {
+    const uint8_t *codes, *scales;
+    const void *dy;
+    int64_t dy_stride;
+    uint64_t rows, rows_per_split; // the latter a multiple of WG_M
+    uint32_t width, out, tiles_k, tiles, splits;
+    float *to; // per split: dw (out, width), then db (out)
+    uint64_t to_stride;
+    float *db; // with one split: db's own place, or NULL
+};
+
+template <typename T, int ACT>
+__global__ __launch_bounds__(WG_THREADS) void weight_grad_kernel(WeightArgs p)
+{
+    constexpr int A = dy_parts<T>, B = act_parts<ACT>, MOST = A > B ? A : B;
+    __shared__ __attribute__((aligned(16))) WgTile ta[A], tb[B];
+    // Blocks go to the 8 dies in turn: the tiles of one range of rows follow each other on one die, whose L2 then
+    // holds the rows for all of them.
+    const uint32_t slot = blockIdx.x / 8, tile = slot % p.tiles, split = slot / p.tiles * 8 + blockIdx.x % 8;
+    if (split >= p.splits)
+        return;
+    const uint32_t n0 = tile / p.tiles_k * WG_N, k0 = tile % p.tiles_k * WG_K;
+    const uint32_t t = threadIdx.x, lane = t & 63, wn = (t >> 6) / 2 * 64, wk = (t >> 6) % 2 * 64;
+    const uint64_t first = split * p.rows_per_split, end = min(p.rows, first + p.rows_per_split);
+    const bool sums_dy = k0 == 0 && wk == 0;
+
+    // what this thread brings of each 32 rows: 2 x 8 values of dy, 16 codes and their scale
+    const T *dy = (const T *)p.dy;
+    const uint32_t ar = t / 16, an = n0 + t % 16 * 8, br = t / 8, bk = k0 + t % 8 * 16;
+    const uint32_t an_left = an < p.out ? p.out - an : 0, bk_left = bk < p.width ? p.width - bk : 0;
+    const uint32_t blocks = mx_blocks(p.width);
+    float a[2][8];
+    uint32_t code[4], scale = 0;
+    auto bring = [&](uint64_t m0) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint64_t m = m0 + ar + 16 * h;
+            load_upto8(dy + (int64_t)m * p.dy_stride + an, m < end ? an_left : 0, a[h]);
+        }
+        const uint64_t m = m0 + br;
+        const uint32_t n = m < end ? bk_left : 0;
+        const uint8_t *c = p.codes + m * p.width + bk;
+        if (n >= 16) {
+            const u32x4 q = *reinterpret_cast<const u32x4_any *>(c);
+            for (int i = 0; i < 4; ++i)
+                code[i] = q[i];
+        } else {
+            load_codes(c, n, code);
+            load_codes(c + 8, n > 8 ? n - 8 : 0, code + 2);
+        }
+        scale = n ? p.scales[m * blocks + bk / MX_BLOCK] : 0;
+    };
+
+    f32x4 acc[4][4] = {}, sum[4] = {};
+    bf16x8 ones;
+    for (int i = 0; i < 8; ++i)
+        ones[i] = (__bf16)1.0f;
+    if (first < end)
+        bring(first);
+    for (uint64_t m0 = first; m0 < end; m0 += WG_M) {
+        __syncthreads(); // the tiles have been read
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            store_parts<A>(ta, ar + 16 * h, t % 16 * 8, a[h]);
+        const float s = e8m0_value(scale);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float v[8];
+            e4m3_values(code[2 * h], s, v);
+            e4m3_values(code[2 * h + 1], s, v + 4);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                v[i] = act_value<ACT>(v[i]);
+            store_parts<B>(tb, br, t % 8 * 16 + 8 * h, v);
+        }
+        if (m0 + WG_M < end)
+            bring(m0 + WG_M);
+        __syncthreads();
+        bf16x8 x[B][4];
+#pragma unroll
+        for (int j = 0; j < B; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                x[j][k] = read_columns(tb[j], wk + 16 * k, lane);
+#pragma unroll
+        for (int i = 0; i < A; ++i) {
+            bf16x8 y[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+                y[n] = read_columns(ta[i], wn + 16 * n, lane);
+#pragma unroll
+            for (int j = 0; j < B; ++j)
+                if (i + j < MOST)
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            acc[n][k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y[n], x[j][k], acc[n][k], 0, 0, 0);
+            if (sums_dy)
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+                    sum[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y[n], ones, sum[n], 0, 0, 0);
+        }
+    }
+    // a lane holds rows 4 (lane / 16) + i and column lane % 16 of each 16x16
+    float *to = p.to + split * p.to_stride;
+    float *db = p.db ? p.db : p.splits > 1 ? to + (uint64_t)p.out * p.width : nullptr;
+    const uint32_t nn = n0 + wn + 4 * (lane >> 4), kk = k0 + wk + (lane & 15);
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t o = nn + 16 * n + i;
+            if (o >= p.out)
+                continue;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (kk + 16 * k < p.width)
+                    to[(uint64_t)o * p.width + kk + 16 * k] = acc[n][k][i];
+            if (sums_dy && db && (lane & 15) == 0)
+                db[o] = sum[n][i];
+        }
+}
+
+// Joins the ranges' sums, in their order: 64 sums a block, four runs of ranges
+// side by side.
+__global__ __launch_bounds__(256) void weight_join_kernel(const float *__restrict__ parts, uint32_t splits, uint64_t n,
+                                                          uint64_t total, float *__restrict__ dw, float *__restrict__ db)
+{
+    __shared__ float run[4][64];
+    const uint64_t i = (uint64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+    const uint32_t g = threadIdx.x >> 6, each = (splits + 3) / 4, last = min(splits, (g + 1) * each);
+    float s = 0.0f;
+    if (i < total) {
+#pragma unroll 8
+        for (uint32_t q = g * each; q < last; ++q)
+            s += parts[q * total + i];
+    }
+    run[g][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (g == 0 && i < total) {
+        s = ((run[0][threadIdx.x] + run[1][threadIdx.x]) + run[2][threadIdx.x]) + run[3][threadIdx.x];
+        if (i < n)
+            dw[i] = s;
+        else if (db)
+            db[i - n] = s;
+    }
+}
+
+// Ranges of rows: enough blocks to fill the chip twice over, 128 rows each at least.
 static uint32_t weight_splits(uint64_t rows, uint32_t width, uint32_t out)
 {
-    const uint64_t tiles = (uint64_t)(width / WG_TILE + 1) * (out / WG_TILE + 1);
-    uint64_t s = tiles < 2048 ? 2048 / tiles : 1;
-    const uint64_t most = (rows + 255) / 256;
-    return (uint32_t)(s < most ? s : most ? most : 1);
+    const uint64_t tiles = (uint64_t)(width ? (width + WG_K - 1) / WG_K : 1) * ((out + WG_N - 1) / WG_N);
+    const uint64_t want = (512 + tiles - 1) / tiles, most = (rows + 127) / 128;
+    return (uint32_t)(want < most ? want : most ? most : 1);
 }
 
 template <typename F>
@@ -330,29 +499,37 @@ extern "C" int vt_act_weight_grad(int dtype, int act, const uint8_t *codes, cons
     VT_REQUIRE((dw || width == 0) && ((codes && scales) || rows == 0 || width == 0) && (dy || rows == 0), "null pointer argument");
     const uint32_t splits = weight_splits(rows, width, out);
     VT_REQUIRE(splits == 1 || workspace, "null workspace");
-    const uint64_t n = (uint64_t)out * width, per = ((rows + splits - 1) / splits + WG_ROWS - 1) / WG_ROWS * WG_ROWS;
-    float *pw = splits > 1 ? (float *)workspace : dw, *pb = !db ? nullptr : splits > 1 ? pw + splits * n : db;
-    // without inputs (width 0) the tiles of k = 0 still sum db
-    const dim3 grid(width ? (width + WG_TILE - 1) / WG_TILE : 1, (out + WG_TILE - 1) / WG_TILE, splits);
+    const uint64_t n = (uint64_t)out * width;
+    WeightArgs p{};
+    p.codes = codes;
+    p.scales = scales;
+    p.dy = dy;
+    p.dy_stride = dy_stride;
+    p.rows = rows;
+    p.rows_per_split = ((rows + splits - 1) / splits + WG_M - 1) / WG_M * WG_M;
+    p.width = width;
+    p.out = out;
+    p.tiles_k = width ? (width + WG_K - 1) / WG_K : 1; // without inputs the tile of k = 0 still sums db
+    p.splits = splits;
+    p.to = splits > 1 ? (float *)workspace : dw;
+    p.to_stride = splits > 1 ? n + out : 0;
+    p.db = splits > 1 ? nullptr : db;
+    const uint64_t tiles = (uint64_t)p.tiles_k * ((out + WG_N - 1) / WG_N), grid = (splits + 7) / 8 * 8 * tiles;
+    VT_REQUIRE(grid < (1ull << 31), "weights of %u by %u are too many for one call", out, width);
+    p.tiles = (uint32_t)tiles;
     const hipStream_t s = as_stream(stream);
     int rc = with_type(dtype, [&](auto t) -> int {
         return with_act(act, [&](auto a) -> int {
-            typedef decltype(t) T;
-            weight_grad_kernel<T, decltype(a)::value><<<grid, WG_TILE * WG_TILE, 0, s>>>(
-                codes, scales, (const T *)dy, dy_stride, rows, per, width, out, pw, pb);
+            weight_grad_kernel<decltype(t), decltype(a)::value><<<(uint32_t)grid, WG_THREADS, 0, s>>>(p);
             VT_LAUNCH_CHECK("weight_grad_kernel");
             return VT_OK;
         });
     });
     if (rc || splits == 1)
         return rc;
-    if (n) {
-        weight_join_kernel<<<(uint32_t)((n + 255) / 256), 256, 0, s>>>(pw, splits, n, dw);
-        VT_LAUNCH_CHECK("weight_join_kernel");
-    }
-    if (db) {
-        weight_join_kernel<<<(out + 255) / 256, 256, 0, s>>>(pb, splits, out, db);
-        VT_LAUNCH_CHECK("weight_join_kernel");
-    }
+    const uint64_t join = (n + out + 63) / 64;
+    VT_REQUIRE(join < (1ull << 31), "weights of %u by %u are too many for one call", out, width);
+    weight_join_kernel<<<(uint32_t)join, 256, 0, s>>>(p.to, splits, n, n + out, dw, db);
+    VT_LAUNCH_CHECK("weight_join_kernel");
     return VT_OK;
 }
