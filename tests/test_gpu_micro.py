@@ -252,6 +252,19 @@ def test_weight_grad(gpu, size, dtype, act):
     assert torch.equal(dw, again[0]) and torch.equal(db, again[1])
 
 
+def test_weight_grad_of_tiny_activations(gpu):
+    """Blocks under the smallest scale: values whose bf16 is subnormal (multiples of 2^-133 at least are exact)."""
+    z = (_rows((64, 40), F32, 26, gpu).sign() * 2.0 ** -127).contiguous()
+    z[:, ::3] *= 0.375
+    for act in ("none", "relu"):
+        kept = micro.checkpoint_activation(z, act)[1]
+        assert int(kept.scales.max()) == 0
+        dy = torch.full((64, 8), 2.0 ** 100, device=gpu).bfloat16()
+        dw, _ = kept.weight_grad(dy)
+        a = O.act(O.ckpt8(O.f64(z))[2], act)
+        assert np.array_equal(O.f64(dw), np.broadcast_to(2.0 ** 100 * a.sum(0), (8, 40)))
+
+
 def test_weight_grad_against_differences(gpu):
     """The loss sum(dy * (act(z^) W^T + b)) is linear in W and b: its differences, in 64 bits, are the gradients."""
     z = _rows((50, 40), F32, 15, gpu) / 8

@@ -172,13 +172,20 @@ __global__ __launch_bounds__(ACT_THREADS) void ckpt8_read_kernel(const uint8_t *
 // its bits (f16: 2, f32 and the smooth activations: 3), and the products of
 // parts down to 2^-16 of the first are summed (2, 3, 5 or 6 instructions).
 constexpr int WG_THREADS = 256, WG_N = 128, WG_K = 128, WG_M = 32;
-// 288 bytes a row: the four rows of a transposing read fall into different banks
-constexpr int WG_PITCH = 144;
-
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef uint16_t WgTile[WG_M][WG_PITCH];
+typedef uint16_t WgTile[WG_M][WG_N]; // 256 bytes a row: all 64 banks
+static_assert(WG_N == WG_K, "both operands use WgTile");
+
+// Where (row, col) lies in a tile: the 32-byte pieces of a row are exchanged
+// by the row, so that the rows that a transposing read takes at once, 8 g .. 8
+// g + 3 for two neighbouring g, fall into different banks.
+__device__ __forceinline__ uint32_t wg_at(uint32_t row, uint32_t col)
+{
+    const uint32_t turn = (row & 3) | (row >> 1 & 4);
+    return row * WG_N + (col ^ turn * 16);
+}
 
 template <typename T>
 constexpr int dy_parts = sizeof(T) == 4 ? 3 : std::is_same<T, _Float16>::value ? 2 : 1;
@@ -220,18 +227,80 @@ __device__ __forceinline__ void store_parts(WgTile *tile, uint32_t row, uint32_t
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             w[i] = part[2 * i][p] | (uint32_t)part[2 * i + 1][p] << 16;
-        *reinterpret_cast<u32x4 *>(&tile[p][row][col]) = w;
+        *reinterpret_cast<u32x4 *>(&tile[p][0][0] + wg_at(row, col)) = w;
     }
 }
 
-// A lane's operand: rows 8 g .. 8 g + 7 of column col + lane % 16.
-__device__ __forceinline__ bf16x8 read_columns(WgTile &tile, uint32_t col, uint32_t lane)
+// A lane's operand from rows 8 g .. 8 g + 7 of one column; `at`: wg_at of row
+// 8 g + (lane % 16) / 4 and column 4 (lane % 4) of the 16 columns.
+__device__ __forceinline__ bf16x8 read_columns(WgTile &tile, uint32_t at)
 {
     typedef __attribute__((address_space(3))) s16x4 lds4;
-    const uint32_t i = lane & 15, row = 8 * (lane >> 4) + i / 4, at = col + 4 * (i & 3);
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)&tile[row][at]);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)&tile[row + 4][at]);
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(&tile[0][0] + at));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(&tile[4][0] + at));
     return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// Eight values of dy as they are kept between the load and the tiles: bf16 as
+// it is, wider types in f32.
+template <typename T>
+struct DyPiece {
+    float v[8];
+    __device__ __forceinline__ void load(const T *p, uint32_t n) { load_upto8(p, n, v); }
+    __device__ __forceinline__ void store(WgTile *tile, uint32_t row, uint32_t col)
+    {
+        store_parts<dy_parts<T>>(tile, row, col, v);
+    }
+};
+template <>
+struct DyPiece<__bf16> {
+    u32x4 w;
+    __device__ __forceinline__ void load(const __bf16 *p, uint32_t n)
+    {
+        if (n >= 8) {
+            w = *reinterpret_cast<const u32x4_any *>(p);
+        } else {
+            const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
+            w = u32x4{};
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i)
+                if (i < n)
+                    w[i / 2] |= (uint32_t)h[i] << (16 * (i % 2));
+        }
+    }
+    __device__ __forceinline__ void store(WgTile *tile, uint32_t row, uint32_t col)
+    {
+        *reinterpret_cast<u32x4 *>(&tile[0][0][0] + wg_at(row, col)) = w;
+    }
+};
+
+// Eight e4m3 codes under a scale, through the activation, into the tiles.
+template <int ACT>
+__device__ __forceinline__ void store_activations(WgTile *tile, uint32_t row, uint32_t col, uint32_t c0, uint32_t c1,
+                                                  float scale)
+{
+    if constexpr (act_parts<ACT> == 1) {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        if constexpr (ACT == VT_ACT_RELU) { // the bits of negative codes but their sign (NaN has none): -0
+            const uint32_t n0 = c0 & 0x80808080u, n1 = c1 & 0x80808080u;
+            c0 &= ~(n0 - (n0 >> 7));
+            c1 &= ~(n1 - (n1 >> 7));
+        }
+        u32x4 w;
+        w[0] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)c0, scale, false));
+        w[1] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)c0, scale, true));
+        w[2] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)c1, scale, false));
+        w[3] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)c1, scale, true));
+        *reinterpret_cast<u32x4 *>(&tile[0][0][0] + wg_at(row, col)) = w;
+    } else {
+        float v[8];
+        e4m3_values(c0, scale, v);
+        e4m3_values(c1, scale, v + 4);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = act_value<ACT>(v[i]);
+        store_parts<act_parts<ACT>>(tile, row, col, v);
+    }
 }
 
 struct WeightArgs {
@@ -246,7 +315,7 @@ struct WeightArgs {
 };
 
 template <typename T, int ACT>
-__global__ __launch_bounds__(WG_THREADS) void weight_grad_kernel(WeightArgs p)
+__global__ __launch_bounds__(WG_THREADS, dy_parts<T> + act_parts<ACT> == 2 ? 3 : 2) void weight_grad_kernel(WeightArgs p)
 {
     constexpr int A = dy_parts<T>, B = act_parts<ACT>, MOST = A > B ? A : B;
     __shared__ __attribute__((aligned(16))) WgTile ta[A], tb[B];
@@ -261,69 +330,72 @@ __global__ __launch_bounds__(WG_THREADS) void weight_grad_kernel(WeightArgs p)
     const bool sums_dy = k0 == 0 && wk == 0;
 
     // what this thread brings of each 32 rows: 2 x 8 values of dy, 16 codes and their scale
-    const T *dy = (const T *)p.dy;
     const uint32_t ar = t / 16, an = n0 + t % 16 * 8, br = t / 8, bk = k0 + t % 8 * 16;
     const uint32_t an_left = an < p.out ? p.out - an : 0, bk_left = bk < p.width ? p.width - bk : 0;
     const uint32_t blocks = mx_blocks(p.width);
-    float a[2][8];
-    uint32_t code[4], scale = 0;
-    auto bring = [&](uint64_t m0) {
+    const T *dy = (const T *)p.dy + (int64_t)(first + ar) * p.dy_stride + an;
+    const uint8_t *codes = p.codes + (first + br) * p.width + bk;
+    const uint8_t *scales = p.scales + (first + br) * blocks + bk / MX_BLOCK;
+    // pieces of DEEP steps are on their way at once
+    constexpr int DEEP = A + B == 2 ? 2 : 1;
+    DyPiece<T> a[DEEP][2];
+    uint32_t code[DEEP][4], scale[DEEP];
+    auto bring = [&](uint64_t m0, int d) { // and on by 32 rows
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint64_t m = m0 + ar + 16 * h;
-            load_upto8(dy + (int64_t)m * p.dy_stride + an, m < end ? an_left : 0, a[h]);
-        }
-        const uint64_t m = m0 + br;
-        const uint32_t n = m < end ? bk_left : 0;
-        const uint8_t *c = p.codes + m * p.width + bk;
+        for (int h = 0; h < 2; ++h)
+            a[d][h].load(dy + 16 * h * p.dy_stride, m0 + ar + 16 * h < end ? an_left : 0);
+        const uint32_t n = m0 + br < end ? bk_left : 0;
         if (n >= 16) {
-            const u32x4 q = *reinterpret_cast<const u32x4_any *>(c);
+            const u32x4 q = *reinterpret_cast<const u32x4_any *>(codes);
             for (int i = 0; i < 4; ++i)
-                code[i] = q[i];
+                code[d][i] = q[i];
         } else {
-            load_codes(c, n, code);
-            load_codes(c + 8, n > 8 ? n - 8 : 0, code + 2);
+            load_codes(codes, n, code[d]);
+            load_codes(codes + 8, n > 8 ? n - 8 : 0, code[d] + 2);
         }
-        scale = n ? p.scales[m * blocks + bk / MX_BLOCK] : 0;
+        scale[d] = n ? *scales : 0;
+        dy += WG_M * p.dy_stride;
+        codes += (uint64_t)WG_M * p.width;
+        scales += (uint64_t)WG_M * blocks;
     };
 
+    const uint32_t lane_row = 8 * (lane >> 4) + (lane & 15) / 4, lane_col = 4 * (lane & 3);
+    uint32_t at_a[4], at_b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        at_a[i] = wg_at(lane_row, wn + 16 * i + lane_col);
+        at_b[i] = wg_at(lane_row, wk + 16 * i + lane_col);
+    }
     f32x4 acc[4][4] = {}, sum[4] = {};
     bf16x8 ones;
     for (int i = 0; i < 8; ++i)
         ones[i] = (__bf16)1.0f;
-    if (first < end)
-        bring(first);
-    for (uint64_t m0 = first; m0 < end; m0 += WG_M) {
+    auto step = [&](uint64_t m0, int d) {
         __syncthreads(); // the tiles have been read
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-            store_parts<A>(ta, ar + 16 * h, t % 16 * 8, a[h]);
-        const float s = e8m0_value(scale);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float v[8];
-            e4m3_values(code[2 * h], s, v);
-            e4m3_values(code[2 * h + 1], s, v + 4);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                v[i] = act_value<ACT>(v[i]);
-            store_parts<B>(tb, br, t % 8 * 16 + 8 * h, v);
-        }
-        if (m0 + WG_M < end)
-            bring(m0 + WG_M);
+            a[d][h].store(ta, ar + 16 * h, t % 16 * 8);
+        const float s = e8m0_value(scale[d]);
+        // neighbouring rows take their halves in turn: 8 threads of each then write to different banks
+        const bool odd = br & 1;
+        const uint32_t *c = code[d];
+        store_activations<ACT>(tb, br, t % 8 * 16 + 8 * odd, odd ? c[2] : c[0], odd ? c[3] : c[1], s);
+        store_activations<ACT>(tb, br, t % 8 * 16 + 8 * !odd, odd ? c[0] : c[2], odd ? c[1] : c[3], s);
+        if (m0 + DEEP * WG_M < end)
+            bring(m0 + DEEP * WG_M, d);
         __syncthreads();
         bf16x8 x[B][4];
 #pragma unroll
         for (int j = 0; j < B; ++j)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                x[j][k] = read_columns(tb[j], wk + 16 * k, lane);
+                x[j][k] = read_columns(tb[j], at_b[k]);
 #pragma unroll
         for (int i = 0; i < A; ++i) {
             bf16x8 y[4];
 #pragma unroll
             for (int n = 0; n < 4; ++n)
-                y[n] = read_columns(ta[i], wn + 16 * n, lane);
+                y[n] = read_columns(ta[i], at_a[n]);
 #pragma unroll
             for (int j = 0; j < B; ++j)
                 if (i + j < MOST)
@@ -337,6 +409,16 @@ __global__ __launch_bounds__(WG_THREADS) void weight_grad_kernel(WeightArgs p)
                 for (int n = 0; n < 4; ++n)
                     sum[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y[n], ones, sum[n], 0, 0, 0);
         }
+    };
+#pragma unroll
+    for (int d = 0; d < DEEP; ++d)
+        if (first + d * WG_M < end)
+            bring(first + d * WG_M, d);
+    for (uint64_t m0 = first; m0 < end; m0 += DEEP * WG_M) {
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d)
+            if (m0 + d * WG_M < end)
+                step(m0 + d * WG_M, d);
     }
     // a lane holds rows 4 (lane / 16) + i and column lane % 16 of each 16x16
     float *to = p.to + split * p.to_stride;
@@ -383,11 +465,11 @@ __global__ __launch_bounds__(256) void weight_join_kernel(const float *__restric
     }
 }
 
-// Ranges of rows: enough blocks to fill the chip twice over, 128 rows each at least.
+// Ranges of rows: enough blocks for three on every CU, 128 rows each at least.
 static uint32_t weight_splits(uint64_t rows, uint32_t width, uint32_t out)
 {
     const uint64_t tiles = (uint64_t)(width ? (width + WG_K - 1) / WG_K : 1) * ((out + WG_N - 1) / WG_N);
-    const uint64_t want = (512 + tiles - 1) / tiles, most = (rows + 127) / 128;
+    const uint64_t want = (768 + tiles - 1) / tiles, most = (rows + 127) / 128;
     return (uint32_t)(want < most ? want : most ? most : 1);
 }
 
