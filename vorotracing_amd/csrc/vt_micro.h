@@ -43,10 +43,14 @@ __device__ __forceinline__ uint32_t mx4_scale(uint32_t top)
     return e == 255 ? MX_NAN : e > 2 ? e - 2 : 0;
 }
 
-// Two values over 1 to e2m1, in the low byte: nearest even, held to 6.
-__device__ __forceinline__ uint32_t e2m1_pair(float a, float b)
+// Values over `scale` (an e8m0_value) to e2m1 codes, nearest even, held to 6:
+// eight of them in a word, the first in the low nibble.
+__device__ __forceinline__ uint32_t e2m1_word(const float *v, float scale)
 {
-    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, a, b, 1.0f, 0);
+    uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, v[0], v[1], scale, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], scale, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], scale, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], scale, 3);
 }
 
 // ---- element types: eight consecutive values at a time

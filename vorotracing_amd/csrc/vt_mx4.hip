@@ -29,13 +29,7 @@ __global__ __launch_bounds__(MX_THREADS) void mx4_quantize_kernel(const T *__res
     top = max(top, (uint32_t)__shfl_xor((int)top, 1, 4));
     top = max(top, (uint32_t)__shfl_xor((int)top, 2, 4));
     const uint32_t c = mx4_scale(top);
-    uint32_t word = 0;
-    if (c != MX_NAN) {
-        const float inv = e8m0_inverse(c);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            word |= (e2m1_pair(v[2 * i] * inv, v[2 * i + 1] * inv) & 0xffu) << (8 * i);
-    }
+    const uint32_t word = c == MX_NAN ? 0 : e2m1_word(v, e8m0_value(c));
     reinterpret_cast<uint32_t *>(codes)[at] = word;
     if ((threadIdx.x & 3) == 0)
         scales[at / 4] = (uint8_t)c;
@@ -115,6 +109,329 @@ __global__ __launch_bounds__(64) void mx4_linear_kernel(const uint8_t *__restric
             y[(m0 + r) * out + o] = (Y)v;
         }
     }
+}
+
+// ---- a head in one kernel
+//
+// Between its layers a head's values stay in registers: a wave takes 64 rows
+// through all of them, against weights that a block puts into shared memory
+// once (four layers of 256 by 256 take 140 KB).
+//
+// With the weights as the first operand of the 32x32x64 product, a lane ends
+// with 16 outputs of one row: of 32 outputs (one block of the next layer's
+// input) the lanes l and l + 32 hold one half each, n = 8 (i / 4) + 4 (l / 32)
+// + i % 4 for i = 0 .. 15.  Their largest magnitude, and so the block's scale,
+// is one exchange away.  Packed to codes a half is two registers, and one
+// exchange of registers between the halves of the wave
+// (v_permlane32_swap_b32), for the two blocks of 64 outputs, gives each lane
+// the 32 codes of one block: the next layer's operand.  Its codes are in the
+// order of the two halves, and the weights behind are put into the same order
+// when they are staged: a sum over a block does not mind.
+constexpr int MLP_THREADS = 512, MLP_R = 2; // waves of 64 rows: two operands of 32
+constexpr uint32_t MLP_WIDTH = 256;         // most values between layers: four operands of 64
+
+struct MlpLayer {
+    const uint8_t *codes, *scales;
+    const float *bias;
+    uint32_t width, out;
+    uint32_t at;     // of its tiles in shared memory, then its scales, then its biases
+    uint32_t at_scales, at_bias;
+};
+struct MlpArgs {
+    MlpLayer layer[VT_MX4_MAX_LAYERS];
+    uint32_t layers;
+    const void *x;
+    int64_t x_stride;
+    void *y;
+    uint64_t rows;
+};
+
+// Layout of a layer's weights in shared memory, tiles of 32 outputs by 64
+// inputs: 16 bytes for (tile, pair of blocks, half, output), a word of scales
+// (one byte a pair of blocks) for (tile, half, output), a bias for each output.
+inline __host__ __device__ uint32_t mlp_tiles(uint32_t out) { return (out + 31) / 32; }
+inline __host__ __device__ uint32_t mlp_pairs(uint32_t width) { return (width + 63) / 64; }
+
+__device__ __forceinline__ void mlp_stage(const MlpLayer &l, bool reorder, char *lds)
+{
+    const uint32_t tiles = mlp_tiles(l.out), pairs = mlp_pairs(l.width), blocks = mx_blocks(l.width);
+    for (uint32_t i = threadIdx.x; i < tiles * pairs * 64; i += MLP_THREADS) {
+        const uint32_t r = i & 31, g = i >> 5 & 1, tp = i >> 6, tile = tp / pairs, pair = tp % pairs;
+        const uint32_t n = tile * 32 + r, j = 2 * pair + g;
+        u32x4 w = {};
+        uint32_t c = 127;
+        if (n < l.out && j < blocks) {
+            w = *reinterpret_cast<const u32x4_any *>(l.codes + ((uint64_t)n * blocks + j) * 16);
+            c = l.scales[(uint64_t)n * blocks + j];
+        }
+        if (reorder) { // groups of four codes 0 .. 7 to 0 2 4 6 1 3 5 7
+            const u32x4 q = w;
+            w[0] = (q[0] & 0xffffu) | q[1] << 16;
+            w[1] = (q[2] & 0xffffu) | q[3] << 16;
+            w[2] = q[0] >> 16 | (q[1] & 0xffff0000u);
+            w[3] = q[2] >> 16 | (q[3] & 0xffff0000u);
+        }
+        *reinterpret_cast<u32x4 *>(lds + l.at + i * 16) = w;
+        *reinterpret_cast<uint8_t *>(lds + l.at_scales + ((tile * 2 + g) * 32 + r) * 4 + pair) = (uint8_t)c;
+    }
+    for (uint32_t n = threadIdx.x; n < tiles * 32; n += MLP_THREADS)
+        *reinterpret_cast<float *>(lds + l.at_bias + n * 4) = l.bias && n < l.out ? l.bias[n] : 0.0f;
+}
+
+// One layer's 32 outputs of a tile for the wave's rows: acc = bias + sum.
+template <int PAIRS>
+__device__ __forceinline__ void mlp_tile(const MlpLayer &l, const char *lds, uint32_t tile, const u32x4 h[MLP_R][4],
+                                         const uint32_t hs[MLP_R], f32x16 acc[MLP_R])
+{
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 5;
+    const char *b = lds + l.at_bias + (tile * 32 + 4 * g) * 4;
+    f32x16 init;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const f32x4 v = *reinterpret_cast<const f32x4 *>(b + q * 32);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            init[4 * q + i] = v[i];
+    }
+    const uint32_t ws = *reinterpret_cast<const uint32_t *>(lds + l.at_scales + (tile * 64 + lane) * 4);
+    const char *w = lds + l.at + tile * PAIRS * 1024 + lane * 16;
+    i32x8 a[PAIRS];
+#pragma unroll
+    for (int p = 0; p < PAIRS; ++p) {
+        const u32x4 q = *reinterpret_cast<const u32x4 *>(w + p * 1024);
+        a[p] = i32x8{(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int m = 0; m < MLP_R; ++m) {
+        acc[m] = init;
+#define VT_MLP_STEP(p)                                                                                                 \
+    if constexpr (PAIRS > p) {                                                                                         \
+        const i32x8 v = {(int)h[m][p][0], (int)h[m][p][1], (int)h[m][p][2], (int)h[m][p][3], 0, 0, 0, 0};              \
+        acc[m] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[p], v, acc[m], 4, 4, p, (int)ws, p, (int)hs[m]);    \
+    }
+        VT_MLP_STEP(0)
+        VT_MLP_STEP(1)
+        VT_MLP_STEP(2)
+        VT_MLP_STEP(3)
+#undef VT_MLP_STEP
+    }
+}
+
+// The scale byte of a block from its largest magnitude or NaN, and the float.
+__device__ __forceinline__ uint32_t mlp_scale(float top, float &scale)
+{
+    const uint32_t c = mx4_scale(abs_bits(top));
+    scale = e8m0_value(c);
+    return c;
+}
+
+// Half a block of outputs through ReLU to codes: 16 values, two words.
+__device__ __forceinline__ uint32_t mlp_pack(const f32x16 &acc, uint32_t w[2])
+{
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        v[i] = acc[i];
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        top = __builtin_elementwise_maximum(top, v[i]); // NaN stays
+    const uint32_t t = __builtin_bit_cast(uint32_t, top);
+    const auto other = __builtin_amdgcn_permlane32_swap(t, t, false, false);
+    top = __builtin_elementwise_maximum(__builtin_bit_cast(float, (uint32_t)other[0]),
+                                        __builtin_bit_cast(float, (uint32_t)other[1]));
+    float scale;
+    const uint32_t c = mlp_scale(top, scale);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t q = e2m1_word(v + 8 * i, scale), s = q & 0x88888888u;
+        w[i] = q & ~(s - (s >> 3)); // negative codes to -0
+    }
+    return c;
+}
+
+template <int PAIRS>
+__device__ __forceinline__ void mlp_hidden(const MlpLayer &l, const char *lds, u32x4 h[MLP_R][4], uint32_t hs[MLP_R])
+{
+    const uint32_t pairs = mlp_pairs(l.out), tiles = mlp_tiles(l.out);
+    const bool upper = threadIdx.x & 32;
+    u32x4 to[MLP_R][4] = {};
+    uint32_t to_s[MLP_R] = {};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        if ((uint32_t)q >= pairs)
+            break;
+        uint32_t w[2][MLP_R][2], c[2][MLP_R];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            if (b == 0 || 2u * q + 1 < tiles) {
+                f32x16 acc[MLP_R];
+                mlp_tile<PAIRS>(l, lds, 2 * q + b, h, hs, acc);
+#pragma unroll
+                for (int m = 0; m < MLP_R; ++m)
+                    c[b][m] = mlp_pack(acc[m], w[b][m]);
+            } else {
+#pragma unroll
+                for (int m = 0; m < MLP_R; ++m) {
+                    c[b][m] = 127;
+                    w[b][m][0] = w[b][m][1] = 0;
+                }
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < MLP_R; ++m) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const auto s = __builtin_amdgcn_permlane32_swap(w[0][m][i], w[1][m][i], false, false);
+                to[m][q][i] = s[0];
+                to[m][q][2 + i] = s[1];
+            }
+            to_s[m] |= (upper ? c[1][m] : c[0][m]) << (8 * q);
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MLP_R; ++m) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            h[m][q] = to[m][q];
+        hs[m] = to_s[m];
+    }
+}
+
+template <int PAIRS, typename Y>
+__device__ __forceinline__ void mlp_last(const MlpLayer &l, const char *lds, const u32x4 h[MLP_R][4],
+                                         const uint32_t hs[MLP_R], uint64_t m0, uint64_t rows, Y *y)
+{
+    const uint32_t r = threadIdx.x & 31, g = threadIdx.x >> 5 & 1, tiles = mlp_tiles(l.out);
+    for (uint32_t t = 0; t < tiles; ++t) {
+        f32x16 acc[MLP_R];
+        mlp_tile<PAIRS>(l, lds, t, h, hs, acc);
+#pragma unroll
+        for (int m = 0; m < MLP_R; ++m) {
+            const uint64_t row = m0 + 32 * m + r;
+            // the halves trade runs of four, so that each has eight neighbouring outputs: 16 q + 8 g
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float a0 = acc[m][8 * q + i], a1 = acc[m][8 * q + 4 + i];
+                    const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a0),
+                                                                    __builtin_bit_cast(uint32_t, a1), false, false);
+                    v[i] = __builtin_bit_cast(float, (uint32_t)s[0]);
+                    v[4 + i] = __builtin_bit_cast(float, (uint32_t)s[1]);
+                }
+                const uint32_t n = t * 32 + 16 * q + 8 * g;
+                if (row < rows && n < l.out)
+                    store_upto8(y + row * l.out + n, l.out - n, v);
+            }
+        }
+    }
+}
+
+// Rows of x as operands: a lane's block of 32 of row r, quantised.
+template <typename T>
+__device__ __forceinline__ void mlp_rows(const T *x, int64_t x_stride, uint64_t m0, uint64_t rows, uint32_t width,
+                                         u32x4 h[MLP_R][4], uint32_t hs[MLP_R])
+{
+    const uint32_t r = threadIdx.x & 31, g = threadIdx.x >> 5 & 1, pairs = mlp_pairs(width);
+#pragma unroll
+    for (int m = 0; m < MLP_R; ++m) {
+        const T *row = x + (int64_t)min(m0 + 32 * m + r, rows - 1) * x_stride;
+        hs[m] = 0;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            h[m][p] = u32x4{};
+            if ((uint32_t)p >= pairs)
+                continue;
+            const uint32_t k = 64 * p + 32 * g;
+            float v[32];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i)
+                load_upto8(row + k + 8 * i, k + 8 * i < width ? width - k - 8 * i : 0, v + 8 * i);
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                top = max(top, abs_bits(v[i]));
+            const uint32_t c = mx4_scale(top);
+            const float scale = e8m0_value(c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                h[m][p][i] = e2m1_word(v + 8 * i, scale);
+            hs[m] |= c << (8 * p);
+        }
+    }
+}
+
+template <typename T, typename Y>
+__global__ __launch_bounds__(MLP_THREADS) void mx4_mlp_kernel(MlpArgs p)
+{
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    for (uint32_t i = 0; i < p.layers; ++i)
+        mlp_stage(p.layer[i], i > 0, lds);
+    __syncthreads();
+    // tiles of rows to blocks in turn, so that few of them spread over the chip
+    for (uint64_t tile = blockIdx.x + (uint64_t)(threadIdx.x / 64) * gridDim.x; tile * (32 * MLP_R) < p.rows;
+         tile += (uint64_t)gridDim.x * (MLP_THREADS / 64)) {
+        const uint64_t m0 = tile * (32 * MLP_R);
+        u32x4 h[MLP_R][4];
+        uint32_t hs[MLP_R];
+        mlp_rows((const T *)p.x, p.x_stride, m0, p.rows, p.layer[0].width, h, hs);
+        for (uint32_t i = 0; i + 1 < p.layers; ++i) {
+            const MlpLayer &l = p.layer[i];
+            switch (mlp_pairs(l.width)) {
+            case 1: mlp_hidden<1>(l, lds, h, hs); break;
+            case 2: mlp_hidden<2>(l, lds, h, hs); break;
+            case 3: mlp_hidden<3>(l, lds, h, hs); break;
+            default: mlp_hidden<4>(l, lds, h, hs); break;
+            }
+        }
+        const MlpLayer &l = p.layer[p.layers - 1];
+        switch (mlp_pairs(l.width)) {
+        case 1: mlp_last<1>(l, lds, h, hs, m0, p.rows, (Y *)p.y); break;
+        case 2: mlp_last<2>(l, lds, h, hs, m0, p.rows, (Y *)p.y); break;
+        case 3: mlp_last<3>(l, lds, h, hs, m0, p.rows, (Y *)p.y); break;
+        default: mlp_last<4>(l, lds, h, hs, m0, p.rows, (Y *)p.y); break;
+        }
+    }
+}
+
+// Shared memory that the layers take, and their places in it; 0 where a layer
+// is too wide or the weights do not fit: those heads go layer by layer.
+constexpr uint32_t MLP_LDS = 160 * 1024;
+static uint32_t mlp_places(const vt_mx4_layer *layers, uint32_t num_layers, MlpLayer *to)
+{
+    uint64_t at = 0;
+    for (uint32_t i = 0; i < num_layers; ++i) {
+        const vt_mx4_layer &l = layers[i];
+        if (l.width > MLP_WIDTH || (i + 1 < num_layers && l.out > MLP_WIDTH))
+            return 0;
+        const uint64_t tiles = mlp_tiles(l.out), pairs = mlp_pairs(l.width);
+        const uint64_t scales = at + tiles * pairs * 1024, bias = scales + tiles * 256;
+        if (to)
+            to[i] = MlpLayer{l.codes, l.scales, l.bias, l.width, l.out, (uint32_t)at, (uint32_t)scales, (uint32_t)bias};
+        at = bias + tiles * 128;
+        if (at > MLP_LDS)
+            return 0;
+    }
+    return (uint32_t)at;
+}
+
+static int launch_mlp(int x_dtype, int y_dtype, const MlpArgs &p, uint32_t lds, hipStream_t s)
+{
+    const uint64_t tiles = (p.rows + 32 * MLP_R - 1) / (32 * MLP_R);
+    const uint32_t grid = (uint32_t)(tiles < 256 ? tiles : 256); // one block a CU
+    return with_type(x_dtype, [&](auto t) -> int {
+        return with_type(y_dtype, [&](auto u) -> int {
+            auto kernel = mx4_mlp_kernel<decltype(t), decltype(u)>;
+            if (lds > 65536)
+                VT_HIP_CHECK(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (int)MLP_LDS));
+            kernel<<<grid, MLP_THREADS, lds, s>>>(p);
+            VT_LAUNCH_CHECK("mx4_mlp_kernel");
+            return VT_OK;
+        });
+    });
 }
 
 struct Mx4Rows {
@@ -242,7 +559,7 @@ static void mlp_sizes(uint64_t rows, const vt_mx4_layer *layers, uint32_t num_la
 extern "C" size_t vt_mx4_mlp_workspace_size(int x_dtype, uint64_t rows, const vt_mx4_layer *layers, uint32_t num_layers)
 {
     (void)x_dtype;
-    if (!layers)
+    if (!layers || mlp_places(layers, num_layers, nullptr))
         return 0;
     uint64_t hidden, quant;
     mlp_sizes(rows, layers, num_layers, hidden, quant);
@@ -265,7 +582,17 @@ extern "C" int vt_mx4_mlp(int x_dtype, const void *x, int64_t x_stride, uint64_t
     }
     if (rows == 0)
         return VT_OK;
-    VT_REQUIRE(x && y && workspace, "null pointer argument");
+    VT_REQUIRE(x && y, "null pointer argument");
+    MlpArgs p{};
+    if (const uint32_t lds = mlp_places(layers, num_layers, p.layer)) {
+        p.layers = num_layers;
+        p.x = x;
+        p.x_stride = x_stride;
+        p.y = y;
+        p.rows = rows;
+        return launch_mlp(x_dtype, y_dtype, p, lds, as_stream(stream));
+    }
+    VT_REQUIRE(workspace, "null workspace");
     uint64_t hidden, quant;
     mlp_sizes(rows, layers, num_layers, hidden, quant);
     const uint64_t esize[3] = {4, 2, 2};
