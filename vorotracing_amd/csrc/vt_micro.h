@@ -43,11 +43,19 @@ __device__ __forceinline__ uint32_t mx4_scale(uint32_t top)
     return e == 255 ? MX_NAN : e > 2 ? e - 2 : 0;
 }
 
+// A register of any contents, for instructions that write a part of one.
+__device__ __forceinline__ uint32_t any_word()
+{
+    uint32_t w;
+    asm("" : "=v"(w));
+    return w;
+}
+
 // Values over `scale` (an e8m0_value) to e2m1 codes, nearest even, held to 6:
 // eight of them in a word, the first in the low nibble.
 __device__ __forceinline__ uint32_t e2m1_word(const float *v, float scale)
 {
-    uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, v[0], v[1], scale, 0);
+    uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(any_word(), v[0], v[1], scale, 0);
     w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], scale, 1);
     w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], scale, 2);
     return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], scale, 3);
@@ -131,6 +139,74 @@ __device__ __forceinline__ void store_upto8(T *p, uint32_t n, const float v[8])
                 p[i] = (T)v[i];
     }
 }
+
+// Eight consecutive values as they were loaded, for quantisation to mx4: the
+// largest magnitude and the codes come from 16-bit pairs as they are.
+template <typename T>
+struct Mx4Piece {
+    float v[8];
+    __device__ __forceinline__ void load(const T *p, uint32_t n) { load_upto8(p, n, v); }
+    // bits of an f32 at least as large as any magnitude so far, in the order that mx4_scale takes
+    __device__ __forceinline__ void top(uint32_t &t) const
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            t = max(t, abs_bits(v[i]));
+    }
+    static __device__ __forceinline__ uint32_t top_bits(uint32_t t) { return t; }
+    __device__ __forceinline__ uint32_t word(float scale) const { return e2m1_word(v, scale); }
+};
+template <typename T>
+struct Mx4Piece16 {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    u32x4 w;
+    __device__ __forceinline__ void load(const T *p, uint32_t n)
+    {
+        if (n >= 8) {
+            w = *reinterpret_cast<const u32x4_any *>(p);
+        } else {
+            const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
+            w = u32x4{};
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i)
+                if (i < n)
+                    w[i / 2] |= (uint32_t)h[i] << (16 * (i % 2));
+        }
+    }
+    __device__ __forceinline__ void top(uint32_t &t) const // two running maxima of 16 bits
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            t = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, t),
+                                                                       __builtin_bit_cast(u16x2, (uint32_t)w[i] & 0x7fff7fffu)));
+    }
+    static __device__ __forceinline__ uint32_t top_bits(uint32_t t)
+    {
+        const uint16_t m = (uint16_t)max(t & 0xffffu, t >> 16);
+        return __builtin_bit_cast(uint32_t, (float)__builtin_bit_cast(T, m));
+    }
+};
+template <>
+struct Mx4Piece<__bf16> : Mx4Piece16<__bf16> {
+    __device__ __forceinline__ uint32_t word(float scale) const
+    {
+        uint32_t q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(any_word(), __builtin_bit_cast(t2, (uint32_t)w[0]), scale, 0);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, __builtin_bit_cast(t2, (uint32_t)w[1]), scale, 1);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, __builtin_bit_cast(t2, (uint32_t)w[2]), scale, 2);
+        return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, __builtin_bit_cast(t2, (uint32_t)w[3]), scale, 3);
+    }
+};
+template <>
+struct Mx4Piece<_Float16> : Mx4Piece16<_Float16> {
+    __device__ __forceinline__ uint32_t word(float scale) const
+    {
+        uint32_t q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(any_word(), __builtin_bit_cast(t2, (uint32_t)w[0]), scale, 0);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, __builtin_bit_cast(t2, (uint32_t)w[1]), scale, 1);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, __builtin_bit_cast(t2, (uint32_t)w[2]), scale, 2);
+        return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, __builtin_bit_cast(t2, (uint32_t)w[3]), scale, 3);
+    }
+};
 
 // Host: run a generic lambda with the element type of `dtype`.
 template <typename F>

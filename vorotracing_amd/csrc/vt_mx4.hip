@@ -20,16 +20,15 @@ __global__ __launch_bounds__(MX_THREADS) void mx4_quantize_kernel(const T *__res
     const uint32_t per_row = 4 * mx_blocks(width);
     const uint64_t row = at / per_row;
     const uint32_t k = (uint32_t)(at - row * per_row) * 8;
-    float v[8];
-    load_upto8(x + (int64_t)row * x_stride + k, k < width ? width - k : 0, v);
+    Mx4Piece<T> v;
+    v.load(x + (int64_t)row * x_stride + k, k < width ? width - k : 0);
     uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        top = max(top, abs_bits(v[i]));
+    v.top(top);
+    top = v.top_bits(top);
     top = max(top, (uint32_t)__shfl_xor((int)top, 1, 4));
     top = max(top, (uint32_t)__shfl_xor((int)top, 2, 4));
     const uint32_t c = mx4_scale(top);
-    const uint32_t word = c == MX_NAN ? 0 : e2m1_word(v, e8m0_value(c));
+    const uint32_t word = c == MX_NAN ? 0 : v.word(e8m0_value(c));
     reinterpret_cast<uint32_t *>(codes)[at] = word;
     if ((threadIdx.x & 3) == 0)
         scales[at / 4] = (uint8_t)c;
@@ -149,30 +148,46 @@ struct MlpArgs {
 // Layout of a layer's weights in shared memory, tiles of 32 outputs by 64
 // inputs: 16 bytes for (tile, pair of blocks, half, output), a word of scales
 // (one byte a pair of blocks) for (tile, half, output), a bias for each output.
-inline __host__ __device__ uint32_t mlp_tiles(uint32_t out) { return (out + 31) / 32; }
+// Tiles go by pairs.
 inline __host__ __device__ uint32_t mlp_pairs(uint32_t width) { return (width + 63) / 64; }
+inline __host__ __device__ uint32_t mlp_tiles(uint32_t out) { return 2 * mlp_pairs(out); }
 
 __device__ __forceinline__ void mlp_stage(const MlpLayer &l, bool reorder, char *lds)
 {
     const uint32_t tiles = mlp_tiles(l.out), pairs = mlp_pairs(l.width), blocks = mx_blocks(l.width);
-    for (uint32_t i = threadIdx.x; i < tiles * pairs * 64; i += MLP_THREADS) {
-        const uint32_t r = i & 31, g = i >> 5 & 1, tp = i >> 6, tile = tp / pairs, pair = tp % pairs;
-        const uint32_t n = tile * 32 + r, j = 2 * pair + g;
-        u32x4 w = {};
-        uint32_t c = 127;
-        if (n < l.out && j < blocks) {
-            w = *reinterpret_cast<const u32x4_any *>(l.codes + ((uint64_t)n * blocks + j) * 16);
-            c = l.scales[(uint64_t)n * blocks + j];
+    const uint32_t units = tiles * pairs * 64;
+    constexpr uint32_t EACH = 4; // loads of a thread at once
+    for (uint32_t i0 = threadIdx.x; i0 < units; i0 += EACH * MLP_THREADS) {
+        u32x4 w[EACH];
+        uint32_t c[EACH], at[EACH];
+#pragma unroll
+        for (uint32_t e = 0; e < EACH; ++e) {
+            const uint32_t i = i0 + e * MLP_THREADS;
+            const uint32_t r = i & 31, g = i >> 5 & 1, tp = i >> 6, tile = tp / pairs, pair = tp - tile * pairs;
+            const uint32_t n = tile * 32 + r, j = 2 * pair + g;
+            w[e] = u32x4{};
+            c[e] = 127;
+            at[e] = ((tile * 2 + g) * 32 + r) * 4 + pair;
+            if (i < units && n < l.out && j < blocks) {
+                w[e] = *reinterpret_cast<const u32x4_any *>(l.codes + ((uint64_t)n * blocks + j) * 16);
+                c[e] = l.scales[(uint64_t)n * blocks + j];
+            }
         }
-        if (reorder) { // groups of four codes 0 .. 7 to 0 2 4 6 1 3 5 7
-            const u32x4 q = w;
-            w[0] = (q[0] & 0xffffu) | q[1] << 16;
-            w[1] = (q[2] & 0xffffu) | q[3] << 16;
-            w[2] = q[0] >> 16 | (q[1] & 0xffff0000u);
-            w[3] = q[2] >> 16 | (q[3] & 0xffff0000u);
+#pragma unroll
+        for (uint32_t e = 0; e < EACH; ++e) {
+            const uint32_t i = i0 + e * MLP_THREADS;
+            if (i >= units)
+                break;
+            if (reorder) { // groups of four codes 0 .. 7 to 0 2 4 6 1 3 5 7
+                const u32x4 q = w[e];
+                w[e][0] = (q[0] & 0xffffu) | q[1] << 16;
+                w[e][1] = (q[2] & 0xffffu) | q[3] << 16;
+                w[e][2] = q[0] >> 16 | (q[1] & 0xffff0000u);
+                w[e][3] = q[2] >> 16 | (q[3] & 0xffff0000u);
+            }
+            *reinterpret_cast<u32x4 *>(lds + l.at + i * 16) = w[e];
+            *reinterpret_cast<uint8_t *>(lds + l.at_scales + at[e]) = (uint8_t)c[e];
         }
-        *reinterpret_cast<u32x4 *>(lds + l.at + i * 16) = w;
-        *reinterpret_cast<uint8_t *>(lds + l.at_scales + ((tile * 2 + g) * 32 + r) * 4 + pair) = (uint8_t)c;
     }
     for (uint32_t n = threadIdx.x; n < tiles * 32; n += MLP_THREADS)
         *reinterpret_cast<float *>(lds + l.at_bias + n * 4) = l.bias && n < l.out ? l.bias[n] : 0.0f;
@@ -217,84 +232,88 @@ __device__ __forceinline__ void mlp_tile(const MlpLayer &l, const char *lds, uin
     }
 }
 
-// The scale byte of a block from its largest magnitude or NaN, and the float.
-__device__ __forceinline__ uint32_t mlp_scale(float top, float &scale)
+// The largest of 16 outputs and 0; NaN stays.
+__device__ __forceinline__ uint32_t mlp_top(const f32x16 &v)
 {
-    const uint32_t c = mx4_scale(abs_bits(top));
-    scale = e8m0_value(c);
-    return c;
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        top = __builtin_elementwise_maximum(top, (float)v[i]);
+    return __builtin_bit_cast(uint32_t, top);
 }
 
-// Half a block of outputs through ReLU to codes: 16 values, two words.
-__device__ __forceinline__ uint32_t mlp_pack(const f32x16 &acc, uint32_t w[2])
+// 16 outputs through ReLU to codes, two words.
+__device__ __forceinline__ void mlp_codes(const f32x16 &acc, float scale, uint32_t w[2])
 {
     float v[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i)
         v[i] = acc[i];
-    float top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-        top = __builtin_elementwise_maximum(top, v[i]); // NaN stays
-    const uint32_t t = __builtin_bit_cast(uint32_t, top);
-    const auto other = __builtin_amdgcn_permlane32_swap(t, t, false, false);
-    top = __builtin_elementwise_maximum(__builtin_bit_cast(float, (uint32_t)other[0]),
-                                        __builtin_bit_cast(float, (uint32_t)other[1]));
-    float scale;
-    const uint32_t c = mlp_scale(top, scale);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const uint32_t q = e2m1_word(v + 8 * i, scale), s = q & 0x88888888u;
         w[i] = q & ~(s - (s >> 3)); // negative codes to -0
     }
-    return c;
 }
 
-template <int PAIRS>
+// 64 outputs of the wave's rows, half of a block and half of another in each
+// lane, through ReLU to the next layer's operand: the lower lanes get the first
+// block and its scale, the upper ones the second.
+__device__ __forceinline__ u32x4 mlp_operand(const f32x16 &a, const f32x16 &b, uint32_t &scale)
+{
+    const auto t = __builtin_amdgcn_permlane32_swap(mlp_top(a), mlp_top(b), false, false);
+    const float top = __builtin_elementwise_maximum(__builtin_bit_cast(float, (uint32_t)t[0]),
+                                                    __builtin_bit_cast(float, (uint32_t)t[1]));
+    const uint32_t e = __builtin_bit_cast(uint32_t, top) >> 23 & 255, c = __builtin_elementwise_sub_sat(e, 2u);
+    // under the scale 255 the codes do not count; c = 0 is the subnormal 2^-127
+    const uint32_t f = max(c << 23, 0x00400000u);
+    const auto of = __builtin_amdgcn_permlane32_swap(f, f, false, false); // the first block's for all, the second's
+    uint32_t p[2], q[2];
+    mlp_codes(a, __builtin_bit_cast(float, (uint32_t)of[0]), p);
+    mlp_codes(b, __builtin_bit_cast(float, (uint32_t)of[1]), q);
+    const auto s0 = __builtin_amdgcn_permlane32_swap(p[0], q[0], false, false);
+    const auto s1 = __builtin_amdgcn_permlane32_swap(p[1], q[1], false, false);
+    scale = e == 255 ? MX_NAN : c;
+    return u32x4{s0[0], s1[0], s0[1], s1[1]};
+}
+
+template <int PAIRS, int TO>
 __device__ __forceinline__ void mlp_hidden(const MlpLayer &l, const char *lds, u32x4 h[MLP_R][4], uint32_t hs[MLP_R])
 {
-    const uint32_t pairs = mlp_pairs(l.out), tiles = mlp_tiles(l.out);
-    const bool upper = threadIdx.x & 32;
-    u32x4 to[MLP_R][4] = {};
+    u32x4 to[MLP_R][TO];
     uint32_t to_s[MLP_R] = {};
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        if ((uint32_t)q >= pairs)
-            break;
-        uint32_t w[2][MLP_R][2], c[2][MLP_R];
+    for (int q = 0; q < TO; ++q) {
+        f32x16 acc[2][MLP_R];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            if (b == 0 || 2u * q + 1 < tiles) {
-                f32x16 acc[MLP_R];
-                mlp_tile<PAIRS>(l, lds, 2 * q + b, h, hs, acc);
-#pragma unroll
-                for (int m = 0; m < MLP_R; ++m)
-                    c[b][m] = mlp_pack(acc[m], w[b][m]);
-            } else {
-#pragma unroll
-                for (int m = 0; m < MLP_R; ++m) {
-                    c[b][m] = 127;
-                    w[b][m][0] = w[b][m][1] = 0;
-                }
-            }
+            mlp_tile<PAIRS>(l, lds, 2 * q + b, h, hs, acc[b]);
+            __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int m = 0; m < MLP_R; ++m) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const auto s = __builtin_amdgcn_permlane32_swap(w[0][m][i], w[1][m][i], false, false);
-                to[m][q][i] = s[0];
-                to[m][q][2 + i] = s[1];
-            }
-            to_s[m] |= (upper ? c[1][m] : c[0][m]) << (8 * q);
+            uint32_t c;
+            to[m][q] = mlp_operand(acc[0][m], acc[1][m], c);
+            to_s[m] |= c << (8 * q);
         }
     }
 #pragma unroll
     for (int m = 0; m < MLP_R; ++m) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int q = 0; q < TO; ++q)
             h[m][q] = to[m][q];
         hs[m] = to_s[m];
+    }
+}
+
+template <int PAIRS>
+__device__ __forceinline__ void mlp_hidden(const MlpLayer &l, const char *lds, u32x4 h[MLP_R][4], uint32_t hs[MLP_R])
+{
+    switch (mlp_pairs(l.out)) {
+    case 1: mlp_hidden<PAIRS, 1>(l, lds, h, hs); break;
+    case 2: mlp_hidden<PAIRS, 2>(l, lds, h, hs); break;
+    case 3: mlp_hidden<PAIRS, 3>(l, lds, h, hs); break;
+    default: mlp_hidden<PAIRS, 4>(l, lds, h, hs); break;
     }
 }
 
@@ -302,8 +321,8 @@ template <int PAIRS, typename Y>
 __device__ __forceinline__ void mlp_last(const MlpLayer &l, const char *lds, const u32x4 h[MLP_R][4],
                                          const uint32_t hs[MLP_R], uint64_t m0, uint64_t rows, Y *y)
 {
-    const uint32_t r = threadIdx.x & 31, g = threadIdx.x >> 5 & 1, tiles = mlp_tiles(l.out);
-    for (uint32_t t = 0; t < tiles; ++t) {
+    const uint32_t r = threadIdx.x & 31, g = threadIdx.x >> 5 & 1;
+    for (uint32_t t = 0; t * 32 < l.out; ++t) {
         f32x16 acc[MLP_R];
         mlp_tile<PAIRS>(l, lds, t, h, hs, acc);
 #pragma unroll
@@ -331,36 +350,32 @@ __device__ __forceinline__ void mlp_last(const MlpLayer &l, const char *lds, con
 
 // Rows of x as operands: a lane's block of 32 of row r, quantised.
 template <typename T>
-__device__ __forceinline__ void mlp_rows(const T *x, int64_t x_stride, uint64_t m0, uint64_t rows, uint32_t width,
-                                         u32x4 h[MLP_R][4], uint32_t hs[MLP_R])
+__device__ __forceinline__ void mlp_load(const T *x, int64_t x_stride, uint64_t m0, uint64_t rows, uint32_t width,
+                                         uint32_t pair, Mx4Piece<T> v[MLP_R][4])
 {
-    const uint32_t r = threadIdx.x & 31, g = threadIdx.x >> 5 & 1, pairs = mlp_pairs(width);
+    const uint32_t r = threadIdx.x & 31, k = 64 * pair + (threadIdx.x & 32), left = k < width ? width - k : 0;
 #pragma unroll
     for (int m = 0; m < MLP_R; ++m) {
-        const T *row = x + (int64_t)min(m0 + 32 * m + r, rows - 1) * x_stride;
-        hs[m] = 0;
+        const T *at = x + (int64_t)min(m0 + 32 * m + r, rows - 1) * x_stride + k;
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            h[m][p] = u32x4{};
-            if ((uint32_t)p >= pairs)
-                continue;
-            const uint32_t k = 64 * p + 32 * g;
-            float v[32];
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i)
-                load_upto8(row + k + 8 * i, k + 8 * i < width ? width - k - 8 * i : 0, v + 8 * i);
-            uint32_t top = 0;
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-                top = max(top, abs_bits(v[i]));
-            const uint32_t c = mx4_scale(top);
-            const float scale = e8m0_value(c);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                h[m][p][i] = e2m1_word(v + 8 * i, scale);
-            hs[m] |= c << (8 * p);
-        }
+        for (uint32_t i = 0; i < 4; ++i)
+            v[m][i].load(at + 8 * i, left > 8 * i ? left - 8 * i : 0);
     }
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t mlp_quantize(const Mx4Piece<T> v[4], u32x4 &h)
+{
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        v[i].top(top);
+    const uint32_t c = mx4_scale(Mx4Piece<T>::top_bits(top));
+    const float scale = e8m0_value(c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        h[i] = v[i].word(scale);
+    return c;
 }
 
 template <typename T, typename Y>
@@ -370,13 +385,33 @@ __global__ __launch_bounds__(MLP_THREADS) void mx4_mlp_kernel(MlpArgs p)
     for (uint32_t i = 0; i < p.layers; ++i)
         mlp_stage(p.layer[i], i > 0, lds);
     __syncthreads();
-    // tiles of rows to blocks in turn, so that few of them spread over the chip
-    for (uint64_t tile = blockIdx.x + (uint64_t)(threadIdx.x / 64) * gridDim.x; tile * (32 * MLP_R) < p.rows;
-         tile += (uint64_t)gridDim.x * (MLP_THREADS / 64)) {
-        const uint64_t m0 = tile * (32 * MLP_R);
+    // Tiles of rows to blocks in turn, so that few of them spread over the chip. The first 64 values of the next
+    // tile's rows are on their way while this one's are in the layers.
+    const uint64_t step = (uint64_t)gridDim.x * (MLP_THREADS / 64) * (32 * MLP_R);
+    uint64_t m0 = (blockIdx.x + (uint64_t)(threadIdx.x / 64) * gridDim.x) * (32 * MLP_R);
+    const uint32_t width = p.layer[0].width, pairs = mlp_pairs(width);
+    const T *x = (const T *)p.x;
+    Mx4Piece<T> next[MLP_R][4];
+    if (m0 < p.rows)
+        mlp_load(x, p.x_stride, m0, p.rows, width, 0, next);
+    for (; m0 < p.rows; m0 += step) {
         u32x4 h[MLP_R][4];
         uint32_t hs[MLP_R];
-        mlp_rows((const T *)p.x, p.x_stride, m0, p.rows, p.layer[0].width, h, hs);
+#pragma unroll
+        for (int m = 0; m < MLP_R; ++m)
+            hs[m] = mlp_quantize<T>(next[m], h[m][0]);
+#pragma unroll
+        for (uint32_t q = 1; q < 4; ++q) {
+            if (q < pairs) {
+                Mx4Piece<T> v[MLP_R][4];
+                mlp_load(x, p.x_stride, m0, p.rows, width, q, v);
+#pragma unroll
+                for (int m = 0; m < MLP_R; ++m)
+                    hs[m] |= mlp_quantize<T>(v[m], h[m][q]) << (8 * q);
+            }
+        }
+        if (m0 + step < p.rows)
+            mlp_load(x, p.x_stride, m0 + step, p.rows, width, 0, next);
         for (uint32_t i = 0; i + 1 < p.layers; ++i) {
             const MlpLayer &l = p.layer[i];
             switch (mlp_pairs(l.width)) {
