@@ -65,49 +65,263 @@ __global__ __launch_bounds__(MX_THREADS) void mx4_dequantize_kernel(const uint8_
     store_upto8(out + row * width + k, width - k, v);
 }
 
-// One wave a tile of 32 rows of x by 32 of w, both read where they lie: a
-// lane's operand of the 32x32x64 product is one block of 32 codes of one row,
-// 16 bytes, with its scale.  w is the first operand, so that a lane ends with
-// runs of four neighbouring outputs of one row.
-template <typename Y>
-__global__ __launch_bounds__(64) void mx4_linear_kernel(const uint8_t *__restrict__ x, const uint8_t *__restrict__ xs,
-                                                        uint64_t rows, uint32_t blocks,
-                                                        const uint8_t *__restrict__ w, const uint8_t *__restrict__ ws,
-                                                        uint32_t out, const float *__restrict__ bias, int relu,
-                                                        Y *__restrict__ y)
+// ---- the product y = x w^T + bias
+//
+// All forms use v_mfma_scale_f32_32x32x64 with the weights as the first
+// operand: a lane's operand is one block of 32 codes of one row, 16 bytes,
+// with its scale byte, and a lane ends with 16 outputs of one row of x, in
+// runs of four: n = 8 (i / 4) + 4 (l / 32) + i % 4.
+
+struct Stored; // x's element type where its rows are in 4 bits already
+
+struct LinearArgs {
+    const void *x; // rows x_stride elements apart, or codes
+    const uint8_t *xs;
+    int64_t x_stride;
+    uint64_t rows;
+    const uint8_t *w, *ws;
+    const float *bias;
+    void *y;
+    uint32_t width, out;
+    int relu, y_dtype;
+};
+
+// Block j of a row of x, `blocks` a row: its codes, and its scale byte as the
+// result.  Blocks past the row's end are zeros.
+template <typename T>
+struct RowBlock {
+    static constexpr int BATCH = 8 / sizeof(T);
+    static __device__ __forceinline__ uint32_t get(const LinearArgs &p, uint64_t row, uint32_t j, uint32_t blocks,
+                                                   u32x4 &codes)
+    {
+        const uint32_t k = j * MX_BLOCK, left = k < p.width ? p.width - k : 0;
+        const T *at = (const T *)p.x + (int64_t)row * p.x_stride + k;
+        Mx4Piece<T> v[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+            v[i].load(at + 8 * i, left > 8 * i ? left - 8 * i : 0);
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            v[i].top(top);
+        const uint32_t c = mx4_scale(Mx4Piece<T>::top_bits(top));
+        const float scale = e8m0_value(c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            codes[i] = v[i].word(scale);
+        return c;
+    }
+};
+__device__ __forceinline__ uint32_t stored_block(const uint8_t *codes, const uint8_t *scales, uint64_t row, uint32_t j,
+                                                 uint32_t blocks, u32x4 &to)
 {
-    const uint32_t tiles_n = (out + 31) / 32;
+    if (j >= blocks) {
+        to = u32x4{};
+        return 127;
+    }
+    to = *reinterpret_cast<const u32x4_any *>(codes + (row * blocks + j) * 16);
+    return scales[row * blocks + j];
+}
+template <>
+struct RowBlock<Stored> {
+    static constexpr int BATCH = 0;
+    static __device__ __forceinline__ uint32_t get(const LinearArgs &p, uint64_t row, uint32_t j, uint32_t blocks,
+                                                   u32x4 &codes)
+    {
+        return stored_block((const uint8_t *)p.x, p.xs, row, j, blocks, codes);
+    }
+};
+
+__device__ __forceinline__ i32x8 operand(const u32x4 &q)
+{
+    return i32x8{(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0};
+}
+
+// Eight neighbouring outputs n .. n + 7 of a row, of which those past `out` are dropped.
+__device__ __forceinline__ void store_outputs(const LinearArgs &p, uint64_t row, uint32_t n, float v[8])
+{
+    if (p.relu) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = __builtin_elementwise_maximum(v[i], 0.0f); // NaN stays
+    }
+    if (n >= p.out)
+        return;
+    const uint64_t at = row * p.out + n;
+    if (p.y_dtype == VT_F32)
+        store_upto8((float *)p.y + at, p.out - n, v);
+    else if (p.y_dtype == VT_F16)
+        store_upto8((_Float16 *)p.y + at, p.out - n, v);
+    else
+        store_upto8((__bf16 *)p.y + at, p.out - n, v);
+}
+
+// A lane's 16 outputs of a tile (n0, row): the halves of the wave trade runs
+// of four, so that each lane stores eight neighbouring outputs at once.
+__device__ __forceinline__ void store_tile(const LinearArgs &p, uint64_t row, uint32_t n0, const f32x16 &acc)
+{
+    const uint32_t g = threadIdx.x >> 5 & 1;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float a0 = acc[8 * q + i], a1 = acc[8 * q + 4 + i];
+            const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a0),
+                                                            __builtin_bit_cast(uint32_t, a1), false, false);
+            v[i] = __builtin_bit_cast(float, (uint32_t)s[0]);
+            v[4 + i] = __builtin_bit_cast(float, (uint32_t)s[1]);
+        }
+        if (row < p.rows)
+            store_outputs(p, row, n0 + 16 * q + 8 * g, v);
+    }
+}
+
+// Few rows, up to 32: a block for each 32 outputs, whose waves share the
+// blocks of the width.  Bound by the two trips to memory (operands, then
+// bias) and the launch; the sums of the waves are joined in shared memory.
+constexpr int FEW_THREADS = 512, FEW_WAVES = FEW_THREADS / 64;
+
+template <typename T>
+__global__ __launch_bounds__(FEW_THREADS) void mx4_few_kernel(LinearArgs p)
+{
+    __shared__ __attribute__((aligned(16))) float part[FEW_WAVES][16][64];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, g = lane >> 5;
+    const uint32_t n0 = blockIdx.x * 32, blocks = mx_blocks(p.width);
+    const uint64_t m = min((uint64_t)r, p.rows - 1);
+    const uint32_t n = min(n0 + r, p.out - 1);
+    f32x16 acc = {};
+    for (uint32_t j0 = 2 * wave; j0 < blocks; j0 += 2 * FEW_WAVES) {
+        u32x4 a, b;
+        const uint32_t sa = stored_block(p.w, p.ws, n, j0 + g, blocks, a);
+        const uint32_t sb = RowBlock<T>::get(p, m, j0 + g, blocks, b);
+        acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(a), operand(b), acc, 4, 4, 0, (int)sa, 0, (int)sb);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        part[wave][i][lane] = acc[i];
+    __syncthreads();
+    // a thread joins two outputs of one row
+    static_assert(FEW_THREADS == 512, "two of the 1024 outputs a thread");
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const uint32_t i = wave * 2 + e, o = n0 + 8 * (i / 4) + 4 * g + i % 4;
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < FEW_WAVES; ++w)
+            v += part[w][i][lane];
+        if (o >= p.out || r >= p.rows)
+            continue;
+        v += p.bias ? p.bias[o] : 0.0f;
+        if (p.relu)
+            v = __builtin_elementwise_maximum(v, 0.0f);
+        const uint64_t at = (uint64_t)r * p.out + o;
+        if (p.y_dtype == VT_F32)
+            ((float *)p.y)[at] = v;
+        else if (p.y_dtype == VT_F16)
+            ((_Float16 *)p.y)[at] = (_Float16)v;
+        else
+            ((__bf16 *)p.y)[at] = (__bf16)v;
+    }
+}
+
+// Many rows and weights that fit into shared memory: each wave takes 32 rows,
+// quantised into registers once, through all outputs.  Bound by reading x and
+// writing y.  PAIRS: 64 inputs each, the width rounded up to 64, 128, 256 or 512.
+constexpr int STREAM_THREADS = 512;
+constexpr uint32_t STREAM_LDS = 160 * 1024;
+
+// Shared memory of the weights: tiles of 32 outputs, for each PAIRS KiB of
+// codes, 16 bytes for (pair, half, output), then 8 bytes of scales for (half,
+// output), then a bias for each output.
+inline uint64_t stream_lds(uint32_t pairs, uint32_t out)
+{
+    const uint64_t tiles = (out + 31) / 32;
+    return tiles * (pairs * 1024 + 512 + 128);
+}
+
+template <typename T, int PAIRS>
+__global__ __launch_bounds__(STREAM_THREADS, 4) void mx4_stream_kernel(LinearArgs p)
+{
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const uint32_t tiles = (p.out + 31) / 32, blocks = mx_blocks(p.width);
+    char *lds_s = lds + tiles * (PAIRS * 1024), *lds_b = lds_s + tiles * 512;
+    for (uint32_t i = threadIdx.x; i < tiles * PAIRS * 64; i += STREAM_THREADS) {
+        const uint32_t r = i & 31, g = i >> 5 & 1, pair = i / 64 % PAIRS, tile = i / (64 * PAIRS), n = tile * 32 + r;
+        u32x4 q = {};
+        const uint32_t c = n < p.out ? stored_block(p.w, p.ws, n, 2 * pair + g, blocks, q) : 127;
+        *reinterpret_cast<u32x4 *>(lds + i * 16) = q;
+        *reinterpret_cast<uint8_t *>(lds_s + ((tile * 2 + g) * 32 + r) * 8 + pair) = (uint8_t)c;
+    }
+    for (uint32_t n = threadIdx.x; n < tiles * 32; n += STREAM_THREADS)
+        *reinterpret_cast<float *>(lds_b + n * 4) = p.bias && n < p.out ? p.bias[n] : 0.0f;
+    __syncthreads();
+    const uint32_t lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
+    const uint64_t step = (uint64_t)gridDim.x * (STREAM_THREADS / 64) * 32;
+    for (uint64_t m0 = (blockIdx.x + (uint64_t)(threadIdx.x / 64) * gridDim.x) * 32; m0 < p.rows; m0 += step) {
+        const uint64_t m = min(m0 + r, p.rows - 1);
+        u32x4 h[PAIRS];
+        uint32_t hs[(PAIRS + 3) / 4] = {};
+#pragma unroll
+        for (int q = 0; q < PAIRS; ++q) {
+            hs[q / 4] |= RowBlock<T>::get(p, m, 2 * q + g, blocks, h[q]) << (8 * (q % 4));
+            // 64 registers of loads on their way at most
+            if (RowBlock<T>::BATCH && q % RowBlock<T>::BATCH == RowBlock<T>::BATCH - 1)
+                __builtin_amdgcn_sched_barrier(0);
+        }
+        for (uint32_t t = 0; t < tiles; ++t) {
+            f32x16 acc;
+            const char *b = lds_b + (t * 32 + 4 * g) * 4, *w = lds + (t * PAIRS * 64 + lane) * 16;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 v = *reinterpret_cast<const f32x4 *>(b + q * 32);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    acc[4 * q + i] = v[i];
+            }
+            const u32x2 s = *reinterpret_cast<const u32x2 *>(lds_s + (t * 64 + lane) * 8);
+#define VT_STREAM_STEP(q)                                                                                              \
+    if constexpr (PAIRS > q)                                                                                           \
+        acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(*reinterpret_cast<const u32x4 *>(w + q * 1024)), \
+                                                              operand(h[q]), acc, 4, 4, q % 4, (int)s[q / 4], q % 4,   \
+                                                              (int)hs[q / 4]);
+            VT_STREAM_STEP(0)
+            VT_STREAM_STEP(1)
+            VT_STREAM_STEP(2)
+            VT_STREAM_STEP(3)
+            VT_STREAM_STEP(4)
+            VT_STREAM_STEP(5)
+            VT_STREAM_STEP(6)
+            VT_STREAM_STEP(7)
+#undef VT_STREAM_STEP
+            store_tile(p, m0 + r, t * 32, acc);
+        }
+    }
+}
+
+// Any size: one wave a tile of 32 rows of x by 32 of w, both stored, read
+// where they lie.
+__global__ __launch_bounds__(64) void mx4_linear_kernel(LinearArgs p)
+{
+    const uint32_t tiles_n = (p.out + 31) / 32, blocks = mx_blocks(p.width);
     const uint64_t m0 = (uint64_t)(blockIdx.x / tiles_n) * 32;
     const uint32_t n0 = (blockIdx.x % tiles_n) * 32;
     const uint32_t r = threadIdx.x & 31, g = threadIdx.x >> 5;
-    const uint64_t m = min(m0 + r, rows - 1);
-    const uint32_t n = min(n0 + r, out - 1);
-    f32x16 acc = {};
-    for (uint32_t j0 = 0; j0 < blocks; j0 += 2) {
-        const uint32_t j = j0 + g;
-        u32x4 a = {}, b = {};
-        uint32_t sa = 127, sb = 127;
-        if (j < blocks) {
-            a = *reinterpret_cast<const u32x4_any *>(w + ((uint64_t)n * blocks + j) * 16);
-            b = *reinterpret_cast<const u32x4_any *>(x + (m * blocks + j) * 16);
-            sa = ws[(uint64_t)n * blocks + j];
-            sb = xs[m * blocks + j];
-        }
-        const i32x8 av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
-        const i32x8 bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
-        acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc, 4, 4, 0, (int)sa, 0, (int)sb);
-    }
-    if (m0 + r >= rows)
-        return;
+    const uint64_t m = min(m0 + r, p.rows - 1);
+    const uint32_t n = min(n0 + r, p.out - 1);
+    f32x16 acc;
+#pragma unroll
     for (int i = 0; i < 16; ++i) {
         const uint32_t o = n0 + 8 * (i / 4) + 4 * g + i % 4;
-        if (o < out) {
-            float v = acc[i] + (bias ? bias[o] : 0.0f);
-            if (relu)
-                v = v < 0.0f ? 0.0f : v; // NaN stays
-            y[(m0 + r) * out + o] = (Y)v;
-        }
+        acc[i] = p.bias && o < p.out ? p.bias[o] : 0.0f;
     }
+    for (uint32_t j0 = 0; j0 < blocks; j0 += 2) {
+        u32x4 a, b;
+        const uint32_t sa = stored_block(p.w, p.ws, n, j0 + g, blocks, a);
+        const uint32_t sb = RowBlock<Stored>::get(p, m, j0 + g, blocks, b);
+        acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(a), operand(b), acc, 4, 4, 0, (int)sa, 0, (int)sb);
+    }
+    store_tile(p, m0 + r, n0, acc);
 }
 
 // ---- a head in one kernel
@@ -469,10 +683,6 @@ static int launch_mlp(int x_dtype, int y_dtype, const MlpArgs &p, uint32_t lds, 
     });
 }
 
-struct Mx4Rows {
-    const uint8_t *codes, *scales;
-};
-
 static uint64_t align16(uint64_t n) { return (n + 15) & ~(uint64_t)15; }
 
 static uint64_t mx4_bytes(uint64_t rows, uint32_t width) // codes, then scales
@@ -496,31 +706,74 @@ static int launch_quantize(int dtype, const void *x, int64_t x_stride, uint64_t 
     });
 }
 
-static int launch_linear(Mx4Rows x, uint64_t rows, uint32_t width, Mx4Rows w, uint32_t out, const float *bias, int relu,
-                         int y_dtype, void *y, hipStream_t s)
+// How a product is run.
+enum LinearForm { LINEAR_FEW, LINEAR_STREAM, LINEAR_TILES };
+static uint32_t stream_pairs(uint32_t width) { return width <= 64 ? 1 : width <= 128 ? 2 : width <= 256 ? 4 : 8; }
+static LinearForm linear_form(uint64_t rows, uint32_t width, uint32_t out)
 {
-    const uint64_t grid = (rows + 31) / 32 * ((out + 31) / 32);
-    VT_REQUIRE(grid < (1ull << 31), "%llu rows by %u outputs are too many for one call", (unsigned long long)rows, out);
-    return with_type(y_dtype, [&](auto t) -> int {
-        mx4_linear_kernel<<<(uint32_t)grid, 64, 0, s>>>(x.codes, x.scales, rows, mx_blocks(width), w.codes, w.scales, out,
-                                                        bias, relu, (decltype(t) *)y);
-        VT_LAUNCH_CHECK("mx4_linear_kernel");
-        return VT_OK;
-    });
+    if (rows <= 32)
+        return LINEAR_FEW;
+    if (width <= 512 && stream_lds(stream_pairs(width), out) <= STREAM_LDS)
+        return LINEAR_STREAM;
+    return LINEAR_TILES;
 }
 
-static int linear(int x_dtype, const void *x, int64_t x_stride, const uint8_t *x_scales, uint64_t rows, uint32_t width,
-                  Mx4Rows w, uint32_t out, const float *bias, int relu, int y_dtype, void *y, void *workspace,
-                  hipStream_t s)
+template <typename T, int PAIRS>
+static int launch_stream(const LinearArgs &p, hipStream_t s)
 {
-    Mx4Rows xr{(const uint8_t *)x, x_scales};
-    if (x_dtype != VT_MX4) {
-        uint8_t *codes = (uint8_t *)workspace, *scales = codes + 16 * rows * mx_blocks(width);
-        if (int rc = launch_quantize(x_dtype, x, x_stride, rows, width, codes, scales, s))
-            return rc;
-        xr = Mx4Rows{codes, scales};
+    const uint32_t lds = (uint32_t)stream_lds(PAIRS, p.out);
+    auto kernel = mx4_stream_kernel<T, PAIRS>;
+    if (lds > 65536)
+        VT_HIP_CHECK(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)STREAM_LDS));
+    // a block stays on its CU, which holds two where the weights leave room for both
+    const uint64_t tiles = (p.rows + 31) / 32, most = lds <= STREAM_LDS / 2 ? 512 : 256;
+    kernel<<<(uint32_t)(tiles < most ? tiles : most), STREAM_THREADS, lds, s>>>(p);
+    VT_LAUNCH_CHECK("mx4_stream_kernel");
+    return VT_OK;
+}
+
+template <typename T>
+static int launch_rows(const LinearArgs &p, LinearForm form, hipStream_t s)
+{
+    if (form == LINEAR_FEW) {
+        mx4_few_kernel<T><<<(p.out + 31) / 32, FEW_THREADS, 0, s>>>(p);
+        VT_LAUNCH_CHECK("mx4_few_kernel");
+        return VT_OK;
     }
-    return launch_linear(xr, rows, width, w, out, bias, relu, y_dtype, y, s);
+    switch (stream_pairs(p.width)) {
+    case 1: return launch_stream<T, 1>(p, s);
+    case 2: return launch_stream<T, 2>(p, s);
+    case 4: return launch_stream<T, 4>(p, s);
+    default: return launch_stream<T, 8>(p, s);
+    }
+}
+
+static uint64_t linear_workspace(int x_dtype, uint64_t rows, uint32_t width, uint32_t out)
+{
+    return x_dtype == VT_MX4 || linear_form(rows, width, out) != LINEAR_TILES ? 0 : mx4_bytes(rows, width);
+}
+
+static int linear(int x_dtype, LinearArgs p, void *workspace, hipStream_t s)
+{
+    const LinearForm form = linear_form(p.rows, p.width, p.out);
+    if (form != LINEAR_TILES) {
+        if (x_dtype == VT_MX4)
+            return launch_rows<Stored>(p, form, s);
+        return with_type(x_dtype, [&](auto t) -> int { return launch_rows<decltype(t)>(p, form, s); });
+    }
+    if (x_dtype != VT_MX4) {
+        uint8_t *codes = (uint8_t *)workspace, *scales = codes + 16 * p.rows * mx_blocks(p.width);
+        if (int rc = launch_quantize(x_dtype, p.x, p.x_stride, p.rows, p.width, codes, scales, s))
+            return rc;
+        p.x = codes;
+        p.xs = scales;
+    }
+    const uint64_t grid = (p.rows + 31) / 32 * ((p.out + 31) / 32);
+    VT_REQUIRE(grid < (1ull << 31), "%llu rows by %u outputs are too many for one call", (unsigned long long)p.rows, p.out);
+    mx4_linear_kernel<<<(uint32_t)grid, 64, 0, s>>>(p);
+    VT_LAUNCH_CHECK("mx4_linear_kernel");
+    return VT_OK;
 }
 
 } // namespace vt
@@ -556,8 +809,7 @@ extern "C" int vt_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, ui
 
 extern "C" size_t vt_mx4_linear_workspace_size(int x_dtype, uint64_t rows, uint32_t width, uint32_t out)
 {
-    (void)out;
-    return x_dtype == VT_MX4 ? 0 : mx4_bytes(rows, width);
+    return rows && out ? linear_workspace(x_dtype, rows, width, out) : 0;
 }
 
 extern "C" int vt_mx4_linear(int x_dtype, const void *x, int64_t x_stride, const uint8_t *x_scales, uint64_t rows,
@@ -569,22 +821,23 @@ extern "C" int vt_mx4_linear(int x_dtype, const void *x, int64_t x_stride, const
         return VT_OK;
     VT_REQUIRE(y && ((x && w_codes && w_scales) || width == 0), "null pointer argument");
     VT_REQUIRE(x_dtype != VT_MX4 || x_scales || width == 0, "x in 4 bits needs its scales");
-    VT_REQUIRE(x_dtype == VT_MX4 || workspace || width == 0, "null workspace");
     VT_REQUIRE(x_dtype >= VT_F32 && x_dtype <= VT_MX4, "x dtype %d is none of VT_F32, VT_F16, VT_BF16, VT_MX4", x_dtype);
     VT_REQUIRE(y_dtype >= VT_F32 && y_dtype <= VT_BF16, "y dtype %d is none of VT_F32, VT_F16, VT_BF16", y_dtype);
-    return linear(x_dtype, x, x_stride, x_scales, rows, width, Mx4Rows{w_codes, w_scales}, out, bias, relu, y_dtype, y,
+    VT_REQUIRE(workspace || !linear_workspace(x_dtype, rows, width, out), "null workspace");
+    return linear(x_dtype, LinearArgs{x, x_scales, x_stride, rows, w_codes, w_scales, bias, y, width, out, relu, y_dtype},
                   workspace, as_stream(stream));
 }
 
 // Rows of a head's layers that go through the workspace at once.
 static constexpr uint64_t MLP_CHUNK = 65536;
 
-// {bytes of the hidden values of a chunk (f32, two of them), bytes of a chunk's quantised rows}
+// {bytes of one of two places for the hidden values of a chunk (f32), bytes of a chunk's quantised rows}
 static void mlp_sizes(uint64_t rows, const vt_mx4_layer *layers, uint32_t num_layers, uint64_t &hidden, uint64_t &quant)
 {
     const uint64_t n = rows < MLP_CHUNK ? rows : MLP_CHUNK;
     hidden = quant = 0;
     for (uint32_t i = 0; i < num_layers; ++i) {
+        // a last chunk may be smaller than the others and be run in another form
         const uint64_t q = mx4_bytes(n, layers[i].width), h = i + 1 < num_layers ? align16(4 * n * layers[i].out) : 0;
         quant = q > quant ? q : quant;
         hidden = h > hidden ? h : hidden;
@@ -598,7 +851,7 @@ extern "C" size_t vt_mx4_mlp_workspace_size(int x_dtype, uint64_t rows, const vt
         return 0;
     uint64_t hidden, quant;
     mlp_sizes(rows, layers, num_layers, hidden, quant);
-    return hidden + quant;
+    return 2 * hidden + quant;
 }
 
 extern "C" int vt_mx4_mlp(int x_dtype, const void *x, int64_t x_stride, uint64_t rows, const vt_mx4_layer *layers,
@@ -639,10 +892,10 @@ extern "C" int vt_mx4_mlp(int x_dtype, const void *x, int64_t x_stride, uint64_t
         int type = x_dtype;
         for (uint32_t i = 0; i < num_layers; ++i) {
             const vt_mx4_layer &l = layers[i];
-            void *to = i == last ? (char *)y + m0 * l.out * esize[y_dtype] : (char *)workspace + quant;
-            // the rows are in 4 bits, in the workspace's front, before the product writes over the hidden values
-            if (int rc = linear(type, h, stride, nullptr, n, l.width, Mx4Rows{l.codes, l.scales}, l.out, l.bias,
-                                i != last, i == last ? y_dtype : VT_F32, to, workspace, as_stream(stream)))
+            void *to = i == last ? (char *)y + m0 * l.out * esize[y_dtype] : (char *)workspace + quant + i % 2 * hidden;
+            const LinearArgs args{h,      nullptr, stride, n,     l.codes,   l.scales,
+                                  l.bias, to,      l.width, l.out, i != last, i == last ? y_dtype : (int)VT_F32};
+            if (int rc = linear(type, args, workspace, as_stream(stream)))
                 return rc;
             h = to;
             stride = l.out;
