@@ -2,6 +2,8 @@
 // the way back, the product of two such matrices and a head of such layers.
 #include "vt_micro.h"
 
+#include <type_traits>
+
 namespace vt {
 
 constexpr int MX_THREADS = 256;
@@ -177,6 +179,85 @@ __device__ __forceinline__ void store_tile(const LinearArgs &p, uint64_t row, ui
     }
 }
 
+// A wave's tiles of 32 rows on their way to y, 128 bytes of each row at a time
+// (32 outputs in f32, 64 in 16 bits): they pass through shared memory, so that
+// a store covers whole lines of 8 rows and not 32 bytes of 32.
+constexpr uint32_t OUT_PITCH = 144, OUT_BYTES = 32 * OUT_PITCH; // a wave's place
+
+template <typename Y>
+__device__ __forceinline__ void stage_tile(char *place, uint32_t tile, const f32x16 &acc, int relu)
+{
+    constexpr uint32_t PER = 128 / sizeof(Y); // outputs of a row at a time
+    const uint32_t r = threadIdx.x & 31, g = threadIdx.x >> 5 & 1;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float a0 = acc[8 * q + i], a1 = acc[8 * q + 4 + i];
+            const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a0),
+                                                            __builtin_bit_cast(uint32_t, a1), false, false);
+            v[i] = __builtin_bit_cast(float, (uint32_t)s[0]);
+            v[4 + i] = __builtin_bit_cast(float, (uint32_t)s[1]);
+        }
+        if (relu) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                v[i] = __builtin_elementwise_maximum(v[i], 0.0f); // NaN stays
+        }
+        Elem<Y>::store8((Y *)(place + r * OUT_PITCH) + (tile * 32 % PER + 16 * q + 8 * g), v);
+    }
+}
+
+template <typename Y>
+__device__ __forceinline__ void store_staged(const char *place, Y *y, uint64_t m0, uint64_t rows, uint32_t n0,
+                                             uint32_t out)
+{
+    constexpr uint32_t EACH = 16 / sizeof(Y);
+    const uint32_t lane = threadIdx.x & 63, c = lane & 7, n = n0 + c * EACH;
+    if (n >= out)
+        return;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+        const uint32_t r = lane / 8 + 8 * j;
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(place + r * OUT_PITCH + c * 16);
+        if (m0 + r >= rows)
+            continue;
+        Y *to = y + (m0 + r) * out + n;
+        if (n + EACH <= out) {
+            *reinterpret_cast<u32x4_any *>(to) = w;
+        } else {
+            typedef Y yv __attribute__((ext_vector_type(16 / sizeof(Y))));
+            const yv v = __builtin_bit_cast(yv, w);
+#pragma unroll
+            for (uint32_t i = 0; i < EACH; ++i)
+                if (n + i < out)
+                    to[i] = v[i];
+        }
+    }
+}
+
+// Between a wave's writes to its place and its reads, and back: the same wave's
+// accesses to shared memory are done in order, so this holds the compiler only.
+__device__ __forceinline__ void wave_order()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <typename Y>
+__device__ __forceinline__ void put_tile(char *place, uint32_t tile, uint32_t tiles, const f32x16 &acc, int relu, void *y,
+                                         uint64_t m0, uint64_t rows, uint32_t out)
+{
+    constexpr uint32_t TILES = 4 / sizeof(Y); // of 32 outputs in 128 bytes
+    stage_tile<Y>(place, tile, acc, relu);
+    if (tile % TILES == TILES - 1 || tile + 1 == tiles) {
+        wave_order();
+        store_staged<Y>(place, (Y *)y, m0, rows, tile / TILES * TILES * 32, out);
+        wave_order();
+    }
+}
+
 // Few rows, up to 32: a block for each 32 outputs, whose waves share the
 // blocks of the width.  Bound by the two trips to memory (operands, then
 // bias) and the launch; the sums of the waves are joined in shared memory.
@@ -233,15 +314,19 @@ constexpr uint32_t STREAM_LDS = 160 * 1024;
 
 // Shared memory of the weights: tiles of 32 outputs, for each PAIRS KiB of
 // codes, 16 bytes for (pair, half, output), then 8 bytes of scales for (half,
-// output), then a bias for each output.
+// output), then a bias for each output, then the waves' places for y.
 inline uint64_t stream_lds(uint32_t pairs, uint32_t out)
 {
     const uint64_t tiles = (out + 31) / 32;
-    return tiles * (pairs * 1024 + 512 + 128);
+    return tiles * (pairs * 1024 + 512 + 128) + STREAM_THREADS / 64 * OUT_BYTES;
 }
 
+// Blocks that a CU's registers hold at once.
 template <typename T, int PAIRS>
-__global__ __launch_bounds__(STREAM_THREADS, 4) void mx4_stream_kernel(LinearArgs p)
+constexpr int stream_blocks = PAIRS == 8 && !std::is_same<T, Stored>::value ? 1 : 2;
+
+template <typename T, int PAIRS>
+__global__ __launch_bounds__(STREAM_THREADS, (stream_blocks<T, PAIRS> * 2)) void mx4_stream_kernel(LinearArgs p)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const uint32_t tiles = (p.out + 31) / 32, blocks = mx_blocks(p.width);
@@ -257,17 +342,32 @@ __global__ __launch_bounds__(STREAM_THREADS, 4) void mx4_stream_kernel(LinearArg
         *reinterpret_cast<float *>(lds_b + n * 4) = p.bias && n < p.out ? p.bias[n] : 0.0f;
     __syncthreads();
     const uint32_t lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
+    char *place = lds_b + tiles * 128 + threadIdx.x / 64 * OUT_BYTES;
     const uint64_t step = (uint64_t)gridDim.x * (STREAM_THREADS / 64) * 32;
     for (uint64_t m0 = (blockIdx.x + (uint64_t)(threadIdx.x / 64) * gridDim.x) * 32; m0 < p.rows; m0 += step) {
         const uint64_t m = min(m0 + r, p.rows - 1);
         u32x4 h[PAIRS];
         uint32_t hs[(PAIRS + 3) / 4] = {};
+        if (std::is_same<T, Stored>::value && PAIRS >= 4 && blocks == 2 * PAIRS) {
+            // whole rows: a row's scales come as words, of whose bytes a lane takes the even or the odd ones
+            const u32x2_any *row = reinterpret_cast<const u32x2_any *>(p.xs + m * blocks);
 #pragma unroll
-        for (int q = 0; q < PAIRS; ++q) {
-            hs[q / 4] |= RowBlock<T>::get(p, m, 2 * q + g, blocks, h[q]) << (8 * (q % 4));
-            // 64 registers of loads on their way at most
-            if (RowBlock<T>::BATCH && q % RowBlock<T>::BATCH == RowBlock<T>::BATCH - 1)
-                __builtin_amdgcn_sched_barrier(0);
+            for (int q = 0; q < PAIRS / 4; ++q) {
+                const u32x2 w = row[q];
+                hs[q] = __builtin_amdgcn_perm(w[1], w[0], g ? 0x07050301u : 0x06040200u);
+            }
+#pragma unroll
+            for (int q = 0; q < PAIRS; ++q)
+                h[q] = *reinterpret_cast<const u32x4_any *>((const uint8_t *)p.x + (m * blocks + 2 * q + g) * 16);
+        } else {
+#pragma unroll
+            for (int q = 0; q < PAIRS; ++q) {
+                hs[q / 4] |= RowBlock<T>::get(p, m, 2 * q + g, blocks, h[q]) << (8 * (q % 4));
+                // 64 registers of loads on their way at most
+                if constexpr (RowBlock<T>::BATCH != 0)
+                    if (q % RowBlock<T>::BATCH == RowBlock<T>::BATCH - 1)
+                        asm volatile("" : "+v"(h[q]), "+v"(hs[q / 4])::"memory");
+            }
         }
         for (uint32_t t = 0; t < tiles; ++t) {
             f32x16 acc;
@@ -294,7 +394,12 @@ __global__ __launch_bounds__(STREAM_THREADS, 4) void mx4_stream_kernel(LinearArg
             VT_STREAM_STEP(6)
             VT_STREAM_STEP(7)
 #undef VT_STREAM_STEP
-            store_tile(p, m0 + r, t * 32, acc);
+            if (p.y_dtype == VT_F32)
+                put_tile<float>(place, t, tiles, acc, p.relu, p.y, m0, p.rows, p.out);
+            else if (p.y_dtype == VT_F16)
+                put_tile<_Float16>(place, t, tiles, acc, p.relu, p.y, m0, p.rows, p.out);
+            else
+                put_tile<__bf16>(place, t, tiles, acc, p.relu, p.y, m0, p.rows, p.out);
         }
     }
 }
@@ -727,7 +832,7 @@ static int launch_stream(const LinearArgs &p, hipStream_t s)
         VT_HIP_CHECK(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)STREAM_LDS));
     // a block stays on its CU, which holds two where the weights leave room for both
-    const uint64_t tiles = (p.rows + 31) / 32, most = lds <= STREAM_LDS / 2 ? 512 : 256;
+    const uint64_t tiles = (p.rows + 31) / 32, most = stream_blocks<T, PAIRS> == 2 && lds <= STREAM_LDS / 2 ? 512 : 256;
     kernel<<<(uint32_t)(tiles < most ? tiles : most), STREAM_THREADS, lds, s>>>(p);
     VT_LAUNCH_CHECK("mx4_stream_kernel");
     return VT_OK;
