@@ -139,53 +139,14 @@ __device__ __forceinline__ i32x8 operand(const u32x4 &q)
     return i32x8{(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0};
 }
 
-// Eight neighbouring outputs n .. n + 7 of a row, of which those past `out` are dropped.
-__device__ __forceinline__ void store_outputs(const LinearArgs &p, uint64_t row, uint32_t n, float v[8])
-{
-    if (p.relu) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = __builtin_elementwise_maximum(v[i], 0.0f); // NaN stays
-    }
-    if (n >= p.out)
-        return;
-    const uint64_t at = row * p.out + n;
-    if (p.y_dtype == VT_F32)
-        store_upto8((float *)p.y + at, p.out - n, v);
-    else if (p.y_dtype == VT_F16)
-        store_upto8((_Float16 *)p.y + at, p.out - n, v);
-    else
-        store_upto8((__bf16 *)p.y + at, p.out - n, v);
-}
-
-// A lane's 16 outputs of a tile (n0, row): the halves of the wave trade runs
-// of four, so that each lane stores eight neighbouring outputs at once.
-__device__ __forceinline__ void store_tile(const LinearArgs &p, uint64_t row, uint32_t n0, const f32x16 &acc)
-{
-    const uint32_t g = threadIdx.x >> 5 & 1;
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        float v[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float a0 = acc[8 * q + i], a1 = acc[8 * q + 4 + i];
-            const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a0),
-                                                            __builtin_bit_cast(uint32_t, a1), false, false);
-            v[i] = __builtin_bit_cast(float, (uint32_t)s[0]);
-            v[4 + i] = __builtin_bit_cast(float, (uint32_t)s[1]);
-        }
-        if (row < p.rows)
-            store_outputs(p, row, n0 + 16 * q + 8 * g, v);
-    }
-}
-
 // A wave's tiles of 32 rows on their way to y, 128 bytes of each row at a time
 // (32 outputs in f32, 64 in 16 bits): they pass through shared memory, so that
 // a store covers whole lines of 8 rows and not 32 bytes of 32.
 constexpr uint32_t OUT_PITCH = 144, OUT_BYTES = 32 * OUT_PITCH; // a wave's place
 
 template <typename Y>
-__device__ __forceinline__ void stage_tile(char *place, uint32_t tile, const f32x16 &acc, int relu)
+__device__ __forceinline__ void stage_tile(char *place, uint32_t tile, const f32x16 &acc, int relu,
+                                           const float *bias = nullptr, uint32_t n0 = 0, uint32_t out = 0)
 {
     constexpr uint32_t PER = 128 / sizeof(Y); // outputs of a row at a time
     const uint32_t r = threadIdx.x & 31, g = threadIdx.x >> 5 & 1;
@@ -199,6 +160,14 @@ __device__ __forceinline__ void stage_tile(char *place, uint32_t tile, const f32
                                                             __builtin_bit_cast(uint32_t, a1), false, false);
             v[i] = __builtin_bit_cast(float, (uint32_t)s[0]);
             v[4 + i] = __builtin_bit_cast(float, (uint32_t)s[1]);
+        }
+        if (bias) {
+            const uint32_t n = n0 + 16 * q + 8 * g;
+            float b[8];
+            load_upto8(bias + n, n < out ? out - n : 0, b);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                v[i] += b[i];
         }
         if (relu) {
 #pragma unroll
@@ -404,29 +373,207 @@ __global__ __launch_bounds__(STREAM_THREADS, (stream_blocks<T, PAIRS> * 2)) void
     }
 }
 
-// Any size: one wave a tile of 32 rows of x by 32 of w, both stored, read
-// where they lie.
-__global__ __launch_bounds__(64) void mx4_linear_kernel(LinearArgs p)
-{
-    const uint32_t tiles_n = (p.out + 31) / 32, blocks = mx_blocks(p.width);
-    const uint64_t m0 = (uint64_t)(blockIdx.x / tiles_n) * 32;
-    const uint32_t n0 = (blockIdx.x % tiles_n) * 32;
-    const uint32_t r = threadIdx.x & 31, g = threadIdx.x >> 5;
-    const uint64_t m = min(m0 + r, p.rows - 1);
-    const uint32_t n = min(n0 + r, p.out - 1);
-    f32x16 acc;
+// Any size, both operands stored: a block's tile of 64 WM rows by 32 NT WN
+// outputs, each wave 64 rows by 32 NT outputs of it.  256 inputs (8 blocks) of
+// both sides at a time go straight into shared memory
+// (global_load_lds_dwordx4), the next ones while these are multiplied.  Bound
+// by the matrix products; 16 rows of 128 bytes are read from shared memory at
+// once, so the eight blocks of a row lie in an order of their own, by (row / 2).
+constexpr uint32_t TILE_BLOCKS = 8, TILE_ROW = 16 * TILE_BLOCKS;
+
+template <int WM, int WN, int NT>
+struct TileShape {
+    static constexpr uint32_t M = 64 * WM, N = 32 * NT * WN, WAVES = WM * WN, THREADS = 64 * WAVES;
+    static constexpr uint32_t STAGE = (M + N) * (TILE_ROW + TILE_BLOCKS); // codes of both, then scales of both
+    static constexpr uint32_t LDS = 2 * STAGE;
+    static_assert(WAVES * OUT_BYTES <= LDS, "the waves' places for y reuse the stages");
+};
+
+// One side's rows row0 .. row0 + ROWS - 1 (the last row again past the end).
+template <uint32_t ROWS, uint32_t WAVES>
+struct TileSide {
+    static constexpr uint32_t LOADS = ROWS / 8 / WAVES, SCALES = (ROWS + 64 * WAVES - 1) / (64 * WAVES);
+    static_assert(WAVES % 2 == 0, "a lane's place in the order of blocks is the same in all of its loads");
+    const uint8_t *codes, *scales; // of row0
+    uint32_t blocks, at[LOADS], at_scales[SCALES], place;
+    u32x2 c[SCALES];
+
+    __device__ __forceinline__ void begin(const uint8_t *x, const uint8_t *xs, uint64_t row0, uint64_t rows,
+                                          uint32_t blocks_)
+    {
+        const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, last = (uint32_t)min(rows - 1 - row0, (uint64_t)ROWS);
+        blocks = blocks_;
+        codes = x + row0 * blocks * 16;
+        scales = xs + row0 * blocks;
+        place = (lane & 7) ^ (4 * (wave & 1) | lane / 16); // row / 2 % 8
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const uint32_t o = n0 + 8 * (i / 4) + 4 * g + i % 4;
-        acc[i] = p.bias && o < p.out ? p.bias[o] : 0.0f;
+        for (uint32_t i = 0; i < LOADS; ++i)
+            at[i] = min((i * WAVES + wave) * 8 + lane / 8, last) * blocks * 16 + place * 16;
+#pragma unroll
+        for (uint32_t i = 0; i < SCALES; ++i)
+            at_scales[i] = min(i * 64 * WAVES + threadIdx.x, last) * blocks;
     }
-    for (uint32_t j0 = 0; j0 < blocks; j0 += 2) {
-        u32x4 a, b;
-        const uint32_t sa = stored_block(p.w, p.ws, n, j0 + g, blocks, a);
-        const uint32_t sb = RowBlock<Stored>::get(p, m, j0 + g, blocks, b);
-        acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(a), operand(b), acc, 4, 4, 0, (int)sa, 0, (int)sb);
+
+    // blocks j0 .. j0 + 7, all within the rows: codes to shared memory, scales to registers
+    __device__ __forceinline__ void bring(uint32_t j0, char *to)
+    {
+        const uint32_t wave = threadIdx.x >> 6;
+        // one base for all lanes, and not a pointer of its own for each load
+        j0 = __builtin_amdgcn_readfirstlane(j0);
+        const uint8_t *x = codes + j0 * 16, *xs = scales + j0;
+#pragma unroll
+        for (uint32_t i = 0; i < LOADS; ++i)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(x + at[i]),
+                                             (__attribute__((address_space(3))) void *)(to + (i * WAVES + wave) * 1024),
+                                             16, 0, 0);
+#pragma unroll
+        for (uint32_t i = 0; i < SCALES; ++i)
+            c[i] = *reinterpret_cast<const u32x2_any *>(xs + at_scales[i]);
     }
-    store_tile(p, m0 + r, n0, acc);
+
+    // the rows' last blocks from j0 on, fewer than 8, and zeros behind them
+    __device__ __forceinline__ void bring_last(uint32_t j0, char *to)
+    {
+        const uint32_t wave = threadIdx.x >> 6;
+#pragma unroll
+        for (uint32_t i = 0; i < LOADS; ++i) {
+            u32x4 q = {};
+            if (j0 + place < blocks)
+                q = *reinterpret_cast<const u32x4_any *>(codes + j0 * 16 + at[i]);
+            *reinterpret_cast<u32x4 *>(to + (i * WAVES + wave) * 1024 + (threadIdx.x & 63) * 16) = q;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < SCALES; ++i) {
+            uint64_t v = 0x7f7f7f7f7f7f7f7full;
+#pragma unroll 1
+            for (uint32_t j = 0; j < blocks - j0; ++j)
+                v = (v & ~(255ull << (8 * j))) | (uint64_t)scales[at_scales[i] + j0 + j] << (8 * j);
+            c[i] = __builtin_bit_cast(u32x2, v);
+        }
+    }
+
+    __device__ __forceinline__ void put_scales(char *to) const
+    {
+#pragma unroll
+        for (uint32_t i = 0; i < SCALES; ++i)
+            if (i * 64 * WAVES + threadIdx.x < ROWS)
+                *reinterpret_cast<u32x2 *>(to + (i * 64 * WAVES + threadIdx.x) * 8) = c[i];
+    }
+};
+
+template <int WM, int WN, int NT>
+__global__ __launch_bounds__(64 * WM *WN, 2) void mx4_tile_kernel(LinearArgs p)
+{
+    typedef TileShape<WM, WN, NT> S;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const uint32_t tiles_n = (p.out + S::N - 1) / S::N, blocks = mx_blocks(p.width);
+    // Blocks go to the 8 dies in turn: one die takes all outputs of a range of rows.
+    const uint32_t slot = blockIdx.x / 8;
+    const uint64_t m0 = (uint64_t)(slot / tiles_n * 8 + blockIdx.x % 8) * S::M;
+    const uint32_t n0 = slot % tiles_n * S::N;
+    if (m0 >= p.rows)
+        return;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, g = lane >> 5;
+    const uint32_t wm = wave / WN * 64, wn = wave % WN * (32 * NT);
+
+    TileSide<S::M, S::WAVES> x;
+    TileSide<S::N, S::WAVES> w;
+    x.begin((const uint8_t *)p.x, p.xs, m0, p.rows, blocks);
+    w.begin(p.w, p.ws, n0, p.out, blocks);
+    constexpr uint32_t AT_W = S::M * TILE_ROW, AT_XS = AT_W + S::N * TILE_ROW, AT_WS = AT_XS + S::M * 8;
+    // codes that go straight into shared memory count as loads of the wave that asked for them
+    auto arrived = [] {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
+    f32x16 acc[NT][2] = {};
+    const uint32_t turn = r >> 1 & 7; // rows 32 apart turn alike
+    auto products = [&](const char *stage) {
+        // a lane's scales: its rows' words, of which bytes 0 and 2 are for the blocks g and 2 + g
+        u32x2 ca[2], cb[NT];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+            ca[m] = *reinterpret_cast<const u32x2 *>(stage + AT_XS + (wm + 32 * m + r) * 8) >> (8 * g);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+            cb[n] = *reinterpret_cast<const u32x2 *>(stage + AT_WS + (wn + 32 * n + r) * 8) >> (8 * g);
+        const char *xa = stage + (wm + r) * TILE_ROW, *wa = stage + AT_W + (wn + r) * TILE_ROW;
+#define VT_TILE_STEP(q)                                                                                                \
+    {                                                                                                                  \
+        const uint32_t at = ((2 * q + g) ^ turn) * 16;                                                                 \
+        i32x8 v[2];                                                                                                    \
+        _Pragma("unroll") for (int m = 0; m < 2; ++m) v[m] =                                                           \
+            operand(*reinterpret_cast<const u32x4 *>(xa + m * 32 * TILE_ROW + at));                                    \
+        _Pragma("unroll") for (int n = 0; n < NT; ++n)                                                                 \
+        {                                                                                                              \
+            const i32x8 a = operand(*reinterpret_cast<const u32x4 *>(wa + n * 32 * TILE_ROW + at));                    \
+            _Pragma("unroll") for (int m = 0; m < 2; ++m) acc[n][m] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4( \
+                a, v[m], acc[n][m], 4, 4, 2 * (q & 1), (int)cb[n][q / 2], 2 * (q & 1), (int)ca[m][q / 2]);             \
+        }                                                                                                              \
+    }
+        VT_TILE_STEP(0)
+        VT_TILE_STEP(1)
+        VT_TILE_STEP(2)
+        VT_TILE_STEP(3)
+#undef VT_TILE_STEP
+    };
+    const uint32_t full = blocks / TILE_BLOCKS * TILE_BLOCKS;
+    if (full) {
+        x.bring(0, lds);
+        w.bring(0, lds + AT_W);
+        x.put_scales(lds + AT_XS);
+        w.put_scales(lds + AT_WS);
+        arrived();
+        char *stage = lds, *next = lds + S::STAGE;
+        for (uint32_t j0 = TILE_BLOCKS; j0 < full; j0 += TILE_BLOCKS) {
+            x.bring(j0, next);
+            w.bring(j0, next + AT_W);
+            products(stage);
+            __builtin_amdgcn_sched_barrier(0); // the products do not wait for the next scales
+            x.put_scales(next + AT_XS);
+            w.put_scales(next + AT_WS);
+            arrived(); // and this stage has been read
+            char *t = stage;
+            stage = next;
+            next = t;
+        }
+        products(stage);
+        __syncthreads();
+    }
+    if (full < blocks) {
+        x.bring_last(full, lds);
+        w.bring_last(full, lds + AT_W);
+        x.put_scales(lds + AT_XS);
+        w.put_scales(lds + AT_WS);
+        __syncthreads();
+        products(lds);
+        __syncthreads();
+    }
+    char *place = lds + wave * OUT_BYTES;
+    const uint32_t nw = n0 + wn, left = nw < p.out ? p.out - nw : 0, tiles = min((left + 31) / 32, (uint32_t)NT);
+    auto put = [&](auto y) {
+        typedef decltype(y) Y;
+        constexpr uint32_t TILES = 4 / sizeof(Y); // of 32 outputs in 128 bytes
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (uint32_t t = 0; t < (uint32_t)NT; ++t) {
+                if (t >= tiles)
+                    continue;
+                stage_tile<Y>(place, t, acc[t][m], p.relu, p.bias, nw + 32 * t, p.out);
+                if (t % TILES == TILES - 1 || t + 1 == tiles) {
+                    wave_order();
+                    store_staged<Y>(place, (Y *)p.y, m0 + wm + 32 * m, p.rows, nw + t / TILES * TILES * 32, p.out);
+                    wave_order();
+                }
+            }
+    };
+    if (p.y_dtype == VT_F32)
+        put(float());
+    else if (p.y_dtype == VT_F16)
+        put(_Float16());
+    else
+        put(__bf16());
 }
 
 // ---- a head in one kernel
@@ -854,6 +1001,19 @@ static int launch_rows(const LinearArgs &p, LinearForm form, hipStream_t s)
     }
 }
 
+template <int WM, int WN, int NT>
+static int launch_tiles(const LinearArgs &p, hipStream_t s)
+{
+    typedef TileShape<WM, WN, NT> S;
+    const uint64_t grid = ((p.rows + S::M - 1) / S::M + 7) / 8 * 8 * ((p.out + S::N - 1) / S::N);
+    VT_REQUIRE(grid < (1ull << 31), "%llu rows by %u outputs are too many for one call", (unsigned long long)p.rows, p.out);
+    auto kernel = mx4_tile_kernel<WM, WN, NT>;
+    VT_HIP_CHECK(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::LDS));
+    kernel<<<(uint32_t)grid, S::THREADS, S::LDS, s>>>(p);
+    VT_LAUNCH_CHECK("mx4_tile_kernel");
+    return VT_OK;
+}
+
 static uint64_t linear_workspace(int x_dtype, uint64_t rows, uint32_t width, uint32_t out)
 {
     return x_dtype == VT_MX4 || linear_form(rows, width, out) != LINEAR_TILES ? 0 : mx4_bytes(rows, width);
@@ -874,11 +1034,7 @@ static int linear(int x_dtype, LinearArgs p, void *workspace, hipStream_t s)
         p.x = codes;
         p.xs = scales;
     }
-    const uint64_t grid = (p.rows + 31) / 32 * ((p.out + 31) / 32);
-    VT_REQUIRE(grid < (1ull << 31), "%llu rows by %u outputs are too many for one call", (unsigned long long)p.rows, p.out);
-    mx4_linear_kernel<<<(uint32_t)grid, 64, 0, s>>>(p);
-    VT_LAUNCH_CHECK("mx4_linear_kernel");
-    return VT_OK;
+    return launch_tiles<2, 2, 2>(p, s);
 }
 
 } // namespace vt
