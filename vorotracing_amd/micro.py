@@ -78,11 +78,14 @@ def _same_device(what: str, device, *tensors):
 
 
 def _call(name: str, device, *args):
-    if device.index != torch.cuda.current_device():
+    """The C entry on torch's current stream of the device (its raw handle: a
+    stream object costs as much as the launch)."""
+    index = device.index
+    if index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            _lib.call(name, *args, native._s(device))
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        _lib.call(name, *args, native._s(device))
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _workspace(size: int, device) -> Optional[torch.Tensor]:
@@ -114,6 +117,12 @@ class Mx4:
         blocks = _blocks(width)
         _check_codes("Mx4", codes, scales, 16 * blocks, blocks)
         self.codes, self.scales, self.width = codes, scales, int(width)
+
+    @classmethod
+    def _of(cls, codes, scales, width):  # tensors made here
+        self = cls.__new__(cls)
+        self.codes, self.scales, self.width = codes, scales, width
+        return self
 
     @property
     def shape(self) -> torch.Size:
@@ -153,7 +162,7 @@ def quantize_mx4(x: torch.Tensor) -> Mx4:
     x, rows, stride = _rows(x)
     _call("vt_mx4_quantize", x.device, _DTYPES[x.dtype], x.data_ptr(), stride, rows, width, codes.data_ptr(),
           scales.data_ptr())
-    return Mx4(codes, scales, width)
+    return Mx4._of(codes, scales, width)
 
 
 def _check_layer(what: str, weight, bias, width: int, device):
@@ -252,6 +261,12 @@ class Checkpoint8:
         _check_codes("Checkpoint8", codes, scales, width, _blocks(width))
         self.codes, self.scales, self.activation = codes, scales, activation
 
+    @classmethod
+    def _of(cls, codes, scales, activation):  # tensors made here
+        self = cls.__new__(cls)
+        self.codes, self.scales, self.activation = codes, scales, activation
+        return self
+
     @property
     def shape(self) -> torch.Size:
         return self.codes.shape
@@ -321,7 +336,7 @@ def checkpoint_activation(z: torch.Tensor, activation: str) -> Tuple[torch.Tenso
     src, rows, stride = _rows(z)
     _call("vt_act_checkpoint", z.device, _DTYPES[z.dtype], ACTIVATIONS[activation], src.data_ptr(), stride, rows, width,
           None if activation == "none" else y.data_ptr(), codes.data_ptr(), scales.data_ptr())
-    return y, Checkpoint8(codes, scales, activation)
+    return y, Checkpoint8._of(codes, scales, activation)
 
 
 __all__ = ["Mx4", "quantize_mx4", "linear_mx4", "mlp_mx4", "Checkpoint8", "checkpoint_activation", "ACTIVATIONS"]
