@@ -1,0 +1,155 @@
+"""A ray head: a small network behind the tracer, over what was traced for
+each ray (or stored for each cell), made of the operators of
+``vorotracing_amd.micro``.  No counterpart in the reference.
+
+* ``activated_linear`` is a layer act(z) W^T + b whose backward pass needs only
+  the 8-bit checkpoint of z.
+* ``RayHead`` trains with such layers: a hidden value costs 1.03 bytes between
+  the passes, where autograd keeps 4 (float32) or 2 each for an activation's
+  input and its output.
+* ``RayHeadInfer`` serves it with weights in 4 bits, the whole head in one
+  kernel where its weights fit into shared memory.
+* ``ray_inputs`` makes a head's inputs from traced colours and rays.
+
+``python -m vorotracing_amd.head`` trains a scene and a head together for some
+steps and serves the result.
+"""
+from __future__ import annotations
+
+from typing import Optional, Sequence
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import micro
+
+
+class ActivatedLinear(torch.autograd.Function):
+    """act(z) W^T + b, keeping z in 8 bits (``micro.Checkpoint8``).  With
+    ``four_bit`` the product is the served one, of both sides in 4 bits, and
+    the backward pass takes the rounding for the identity."""
+
+    @staticmethod
+    def forward(ctx, z, weight, bias, activation: str, four_bit: bool):
+        y, kept = micro.checkpoint_activation(z, activation)
+        ctx.save_for_backward(weight, kept.codes, kept.scales)
+        ctx.activation = activation
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.four_bit = four_bit
+        if four_bit:
+            return micro.linear_mx4(y, micro.quantize_mx4(weight), None if bias is None else bias.float())
+        return nn.functional.linear(y, weight.to(z.dtype), None if bias is None else bias.to(z.dtype))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        weight, codes, scales = ctx.saved_tensors
+        kept = micro.Checkpoint8(codes, scales, ctx.activation)
+        dz = dw = db = None
+        if ctx.needs_input_grad[0]:
+            w = micro.quantize_mx4(weight).dequantize(dy.dtype) if ctx.four_bit else weight.to(dy.dtype)
+            dz = kept.input_grad(dy @ w)
+        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+            dw, db = kept.weight_grad(dy)
+            dw = dw.to(weight.dtype) if ctx.needs_input_grad[1] else None
+            db = db.to(ctx.bias_dtype) if ctx.needs_input_grad[2] else None
+        return dz, dw, db, None, None
+
+
+def activated_linear(z: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                     activation: str = "relu", four_bit: bool = False) -> torch.Tensor:
+    """act(z) W^T + b, differentiable in z, W and b: z (..., width) in float32,
+    float16 or bfloat16, the product in z's type, the gradients of W and b
+    summed in float32.  Between the passes only z's 8-bit checkpoint is kept.
+    ``four_bit``: the product of act(z) and W both rounded to 4 bits
+    (``micro.linear_mx4``), whose rounding has the gradient of the identity."""
+    if weight.dim() != 2 or weight.shape[1] != z.shape[-1]:
+        raise ValueError(f"activated_linear: rows of {z.shape[-1]} values with weights of {tuple(weight.shape)}")
+    return ActivatedLinear.apply(z, weight, bias, activation, four_bit)
+
+
+def ray_inputs(rgba: torch.Tensor, rays: torch.Tensor, bands: int = 4) -> torch.Tensor:
+    """Inputs of a head (..., 7 + 6 bands): the traced colour and alpha, the
+    ray's unit direction d, and sin and cos of 2^i pi d for i < bands."""
+    d = torch.nn.functional.normalize(rays[..., 3:6].to(rgba.dtype), dim=-1)
+    turns = d[..., None, :] * (torch.pi * 2.0 ** torch.arange(bands, dtype=rgba.dtype, device=d.device))[:, None]
+    return torch.cat([rgba, d, torch.sin(turns).flatten(-2), torch.cos(turns).flatten(-2)], -1)
+
+
+class RayHead(nn.Module):
+    """Layers of ``widths`` (inputs, hidden ones, outputs) with ``activation``
+    between them, parameters in float32, rows computed in ``dtype``.  A head
+    that is to be served in 4 bits is trained with ``four_bit`` set in its last
+    steps, so that its weights allow for the rounding."""
+
+    def __init__(self, widths: Sequence[int], activation: str = "relu", dtype: torch.dtype = torch.bfloat16,
+                 device=torch.device("cuda")):
+        super().__init__()
+        if len(widths) < 2:
+            raise ValueError("a head has inputs and outputs: two widths at least")
+        if activation not in micro.ACTIVATIONS:
+            raise ValueError(f"activation {activation!r} is none of {', '.join(micro.ACTIVATIONS)}")
+        self.widths, self.activation, self.dtype = tuple(int(w) for w in widths), activation, dtype
+        self.four_bit = False
+        self.layers = nn.ModuleList(nn.Linear(a, b, device=device) for a, b in zip(widths, widths[1:]))
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        h = x.to(self.dtype)
+        for i, layer in enumerate(self.layers):
+            h = activated_linear(h, layer.weight, layer.bias, self.activation if i else "none", self.four_bit)
+        return h
+
+
+class RayHeadInfer:
+    """A trained ``RayHead`` (ReLU) for serving: weights in 4 bits, 0.53 bytes
+    each; ``head(x)`` gives the outputs of the rows of x in x's type or
+    ``dtype``."""
+
+    def __init__(self, head: RayHead):
+        if head.activation != "relu" and len(head.layers) > 1:
+            raise ValueError(f"the 4-bit head runs ReLU between its layers, not {head.activation!r}")
+        self.widths = head.widths
+        with torch.no_grad():
+            self.layers = [(micro.quantize_mx4(layer.weight.detach()),
+                            None if layer.bias is None else layer.bias.detach().float().contiguous().clone())
+                           for layer in head.layers]
+
+    @torch.no_grad()
+    def __call__(self, x: torch.Tensor, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        return micro.mlp_mx4(x.detach(), self.layers, dtype=dtype)
+
+
+def main():
+    """Trains a scene and a head on colours with a view-dependent tint, then serves both."""
+    from . import camera, scene
+    from .infer import VoroTracingInfer
+    from .model import VoroTracing
+
+    torch.manual_seed(0)
+    model = VoroTracing.from_scene(scene.random_scene(4096, seed=1, R=4))
+    rays = torch.from_numpy(camera.pinhole_rays(64, 64, eye=(0.0, -3.5, 0.3))).float().to(model.device)
+    with torch.no_grad():
+        start = model.get_starting_point(rays)
+        rgba = model(rays, start_point=start)[0]
+        target = rgba[..., :3] * (0.5 + 0.5 * torch.nn.functional.normalize(rays[..., 3:], dim=-1) ** 2)
+        inputs = ray_inputs(rgba, rays)
+    head = RayHead([inputs.shape[-1], 64, 64, 3])
+    optimizer = torch.optim.Adam([{"params": head.parameters(), "lr": 2e-3},
+                                  {"params": [model.att_diffuse, model.att_specular], "lr": 1e-3}])
+    for step in range(201):
+        head.four_bit = step > 100
+        optimizer.zero_grad()
+        out = head(ray_inputs(model(rays, start_point=start)[0], rays))
+        loss = (out.float() - target).square().mean()
+        loss.backward()
+        optimizer.step()
+        if step % 50 == 0:
+            print(f"step {step}{' (4 bits)' if head.four_bit else ''}: loss {float(loss.detach()):.6f}", flush=True)
+    infer, serve = VoroTracingInfer(model), RayHeadInfer(head)
+    out = serve(ray_inputs(infer.render(rays).float(), rays))
+    print(f"served in 4 bits: mean squared difference {float((out - target).square().mean()):.6f}")
+
+
+if __name__ == "__main__":
+    main()
