@@ -36,12 +36,17 @@ __global__ __launch_bounds__(MX_THREADS) void mx4_quantize_kernel(const T *__res
         scales[at / 4] = (uint8_t)c;
 }
 
-__device__ __forceinline__ float e2m1_value(uint32_t code)
+// A word of codes under a scale to eight values of T at p (n of them).
+template <typename T>
+__device__ __forceinline__ void put_codes(uint32_t word, float scale, T *p, uint32_t n)
 {
-    // 0, 1/2, 1, 3/2, 2, 3, 4, 6: a float's exponent and top bit, with the subnormal 1/2 apart
-    const uint32_t m = code & 7;
-    const float a = m < 2 ? 0.5f * (float)m : __builtin_bit_cast(float, ((m >> 1) + 126) << 23 | (m & 1) << 22);
-    return code & 8 ? -a : a;
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const f32x2 v0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, scale, 0);
+    const f32x2 v1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, scale, 1);
+    const f32x2 v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, scale, 2);
+    const f32x2 v3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, scale, 3);
+    const float v[8] = {v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
+    store_upto8(p, n, v);
 }
 
 template <typename T>
@@ -59,12 +64,7 @@ __global__ __launch_bounds__(MX_THREADS) void mx4_dequantize_kernel(const uint8_
     if (k >= width)
         return;
     const uint32_t word = reinterpret_cast<const uint32_t *>(codes)[at];
-    const float s = e8m0_value(scales[at / 4]);
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        v[i] = e2m1_value(word >> (4 * i) & 15) * s;
-    store_upto8(out + row * width + k, width - k, v);
+    put_codes(word, e8m0_value(scales[at / 4]), out + row * width + k, width - k);
 }
 
 // ---- the product y = x w^T + bias
