@@ -592,7 +592,7 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void mx4_tile_kernel(LinearArgs p)
 // the 32 codes of one block: the next layer's operand.  Its codes are in the
 // order of the two halves, and the weights behind are put into the same order
 // when they are staged: a sum over a block does not mind.
-constexpr int MLP_THREADS = 512, MLP_R = 2; // waves of 64 rows: two operands of 32
+constexpr int MLP_THREADS = 1024, MLP_R = 1; // waves of 64 rows: two operands of 32
 constexpr uint32_t MLP_WIDTH = 256;         // most values between layers: four operands of 64
 
 struct MlpLayer {
@@ -659,12 +659,22 @@ __device__ __forceinline__ void mlp_stage(const MlpLayer &l, bool reorder, char 
         *reinterpret_cast<float *>(lds + l.at_bias + n * 4) = l.bias && n < l.out ? l.bias[n] : 0.0f;
 }
 
+// The lane's number, and not the compiler's to keep: places in shared memory
+// that follow from it are worked out where they are used, and do not take a
+// register for each form of a layer all the time.
+__device__ __forceinline__ uint32_t lane_here()
+{
+    uint32_t lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+
 // One layer's 32 outputs of a tile for the wave's rows: acc = bias + sum.
 template <int PAIRS>
-__device__ __forceinline__ void mlp_tile(const MlpLayer &l, const char *lds, uint32_t tile, const u32x4 h[MLP_R][4],
+__device__ __forceinline__ void mlp_tile(const MlpLayer &l, const char *lds, uint32_t lane, uint32_t tile, const u32x4 h[MLP_R][4],
                                          const uint32_t hs[MLP_R], f32x16 acc[MLP_R])
 {
-    const uint32_t lane = threadIdx.x & 63, g = lane >> 5;
+    const uint32_t g = lane >> 5;
     const char *b = lds + l.at_bias + (tile * 32 + 4 * g) * 4;
     f32x16 init;
 #pragma unroll
@@ -746,6 +756,7 @@ __device__ __forceinline__ u32x4 mlp_operand(const f32x16 &a, const f32x16 &b, u
 template <int PAIRS, int TO>
 __device__ __forceinline__ void mlp_hidden(const MlpLayer &l, const char *lds, u32x4 h[MLP_R][4], uint32_t hs[MLP_R])
 {
+    const uint32_t lane = lane_here();
     u32x4 to[MLP_R][TO];
     uint32_t to_s[MLP_R] = {};
 #pragma unroll
@@ -753,8 +764,7 @@ __device__ __forceinline__ void mlp_hidden(const MlpLayer &l, const char *lds, u
         f32x16 acc[2][MLP_R];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            mlp_tile<PAIRS>(l, lds, 2 * q + b, h, hs, acc[b]);
-            __builtin_amdgcn_sched_barrier(0);
+            mlp_tile<PAIRS>(l, lds, lane, 2 * q + b, h, hs, acc[b]);
         }
 #pragma unroll
         for (int m = 0; m < MLP_R; ++m) {
@@ -783,14 +793,24 @@ __device__ __forceinline__ void mlp_hidden(const MlpLayer &l, const char *lds, u
     }
 }
 
+__device__ __forceinline__ void mlp_layer(const MlpLayer &l, const char *lds, u32x4 h[MLP_R][4], uint32_t hs[MLP_R])
+{
+    switch (mlp_pairs(l.width)) {
+    case 1: mlp_hidden<1>(l, lds, h, hs); break;
+    case 2: mlp_hidden<2>(l, lds, h, hs); break;
+    case 3: mlp_hidden<3>(l, lds, h, hs); break;
+    default: mlp_hidden<4>(l, lds, h, hs); break;
+    }
+}
+
 template <int PAIRS, typename Y>
 __device__ __forceinline__ void mlp_last(const MlpLayer &l, const char *lds, const u32x4 h[MLP_R][4],
                                          const uint32_t hs[MLP_R], uint64_t m0, uint64_t rows, Y *y)
 {
-    const uint32_t r = threadIdx.x & 31, g = threadIdx.x >> 5 & 1;
+    const uint32_t lane = lane_here(), r = lane & 31, g = lane >> 5;
     for (uint32_t t = 0; t * 32 < l.out; ++t) {
         f32x16 acc[MLP_R];
-        mlp_tile<PAIRS>(l, lds, t, h, hs, acc);
+        mlp_tile<PAIRS>(l, lds, lane, t, h, hs, acc);
 #pragma unroll
         for (int m = 0; m < MLP_R; ++m) {
             const uint64_t row = m0 + 32 * m + r;
@@ -852,20 +872,31 @@ __global__ __launch_bounds__(MLP_THREADS) void mx4_mlp_kernel(MlpArgs p)
         mlp_stage(p.layer[i], i > 0, lds);
     __syncthreads();
     // Tiles of rows to blocks in turn, so that few of them spread over the chip. The first 64 values of the next
-    // tile's rows are on their way while this one's are in the layers.
+    // tile's rows are on their way while this one's are in the first layer, and wait as codes.
     const uint64_t step = (uint64_t)gridDim.x * (MLP_THREADS / 64) * (32 * MLP_R);
     uint64_t m0 = (blockIdx.x + (uint64_t)(threadIdx.x / 64) * gridDim.x) * (32 * MLP_R);
     const uint32_t width = p.layer[0].width, pairs = mlp_pairs(width);
     const T *x = (const T *)p.x;
+    u32x4 first[MLP_R];
+    uint32_t first_s[MLP_R];
     Mx4Piece<T> next[MLP_R][4];
-    if (m0 < p.rows)
+    auto turn = [&] { // the rows that have arrived, to codes
+#pragma unroll
+        for (int m = 0; m < MLP_R; ++m)
+            first_s[m] = mlp_quantize<T>(next[m], first[m]);
+    };
+    if (m0 < p.rows) {
         mlp_load(x, p.x_stride, m0, p.rows, width, 0, next);
+        turn();
+    }
     for (; m0 < p.rows; m0 += step) {
         u32x4 h[MLP_R][4];
         uint32_t hs[MLP_R];
 #pragma unroll
-        for (int m = 0; m < MLP_R; ++m)
-            hs[m] = mlp_quantize<T>(next[m], h[m][0]);
+        for (int m = 0; m < MLP_R; ++m) {
+            h[m][0] = first[m];
+            hs[m] = first_s[m];
+        }
 #pragma unroll
         for (uint32_t q = 1; q < 4; ++q) {
             if (q < pairs) {
@@ -876,17 +907,15 @@ __global__ __launch_bounds__(MLP_THREADS) void mx4_mlp_kernel(MlpArgs p)
                     hs[m] |= mlp_quantize<T>(v[m], h[m][q]) << (8 * q);
             }
         }
-        if (m0 + step < p.rows)
+        const bool more = m0 + step < p.rows;
+        if (more)
             mlp_load(x, p.x_stride, m0 + step, p.rows, width, 0, next);
-        for (uint32_t i = 0; i + 1 < p.layers; ++i) {
-            const MlpLayer &l = p.layer[i];
-            switch (mlp_pairs(l.width)) {
-            case 1: mlp_hidden<1>(l, lds, h, hs); break;
-            case 2: mlp_hidden<2>(l, lds, h, hs); break;
-            case 3: mlp_hidden<3>(l, lds, h, hs); break;
-            default: mlp_hidden<4>(l, lds, h, hs); break;
-            }
-        }
+        if (p.layers > 1)
+            mlp_layer(p.layer[0], lds, h, hs);
+        if (more)
+            turn();
+        for (uint32_t i = 1; i + 1 < p.layers; ++i)
+            mlp_layer(p.layer[i], lds, h, hs);
         const MlpLayer &l = p.layer[p.layers - 1];
         switch (mlp_pairs(l.width)) {
         case 1: mlp_last<1>(l, lds, h, hs, m0, p.rows, (Y *)p.y); break;
