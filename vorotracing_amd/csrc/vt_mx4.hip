@@ -88,6 +88,22 @@ struct LinearArgs {
     int relu, y_dtype;
 };
 
+// A block of 32 as it was loaded to codes; its scale byte is the result.
+template <typename T>
+__device__ __forceinline__ uint32_t quantize_block(const Mx4Piece<T> v[4], u32x4 &codes)
+{
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        v[i].top(top);
+    const uint32_t c = mx4_scale(Mx4Piece<T>::top_bits(top));
+    const float scale = e8m0_value(c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        codes[i] = v[i].word(scale);
+    return c;
+}
+
 // Block j of a row of x, `blocks` a row: its codes, and its scale byte as the
 // result.  Blocks past the row's end are zeros.
 template <typename T>
@@ -102,16 +118,7 @@ struct RowBlock {
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i)
             v[i].load(at + 8 * i, left > 8 * i ? left - 8 * i : 0);
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            v[i].top(top);
-        const uint32_t c = mx4_scale(Mx4Piece<T>::top_bits(top));
-        const float scale = e8m0_value(c);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            codes[i] = v[i].word(scale);
-        return c;
+        return quantize_block(v, codes);
     }
 };
 __device__ __forceinline__ uint32_t stored_block(const uint8_t *codes, const uint8_t *scales, uint64_t row, uint32_t j,
@@ -139,6 +146,20 @@ __device__ __forceinline__ i32x8 operand(const u32x4 &q)
     return i32x8{(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0};
 }
 
+// Outputs 16 q + 8 (l / 32) .. + 7 of a lane's row, of its tile of 32: the
+// halves of the wave trade runs of four.
+__device__ __forceinline__ void eight_outputs(const f32x16 &acc, int q, float v[8])
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float a0 = acc[8 * q + i], a1 = acc[8 * q + 4 + i];
+        const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a0),
+                                                        __builtin_bit_cast(uint32_t, a1), false, false);
+        v[i] = __builtin_bit_cast(float, (uint32_t)s[0]);
+        v[4 + i] = __builtin_bit_cast(float, (uint32_t)s[1]);
+    }
+}
+
 // A wave's tiles of 32 rows on their way to y, 128 bytes of each row at a time
 // (32 outputs in f32, 64 in 16 bits): they pass through shared memory, so that
 // a store covers whole lines of 8 rows and not 32 bytes of 32.
@@ -153,14 +174,7 @@ __device__ __forceinline__ void stage_tile(char *place, uint32_t tile, const f32
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
         float v[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float a0 = acc[8 * q + i], a1 = acc[8 * q + 4 + i];
-            const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a0),
-                                                            __builtin_bit_cast(uint32_t, a1), false, false);
-            v[i] = __builtin_bit_cast(float, (uint32_t)s[0]);
-            v[4 + i] = __builtin_bit_cast(float, (uint32_t)s[1]);
-        }
+        eight_outputs(acc, q, v);
         if (bias) {
             const uint32_t n = n0 + 16 * q + 8 * g;
             float b[8];
@@ -578,7 +592,7 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void mx4_tile_kernel(LinearArgs p)
 
 // ---- a head in one kernel
 //
-// Between its layers a head's values stay in registers: a wave takes 64 rows
+// Between its layers a head's values stay in registers: a wave takes 32 rows
 // through all of them, against weights that a block puts into shared memory
 // once (four layers of 256 by 256 take 140 KB).
 //
@@ -592,8 +606,14 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void mx4_tile_kernel(LinearArgs p)
 // the 32 codes of one block: the next layer's operand.  Its codes are in the
 // order of the two halves, and the weights behind are put into the same order
 // when they are staged: a sum over a block does not mind.
-constexpr int MLP_THREADS = 1024, MLP_R = 1; // waves of 64 rows: two operands of 32
-constexpr uint32_t MLP_WIDTH = 256;         // most values between layers: four operands of 64
+//
+// Bound by the vector instructions that make codes of sums, 33 for 1024 sums
+// of which 8 are conversions at half rate, beside the matrix products.
+//
+// Three waves a SIMD, which leave 168 registers to each: with four, 128, the
+// next rows on their way no longer fit (spills; no faster).
+constexpr uint32_t MLP_THREADS = 768;
+constexpr uint32_t MLP_WIDTH = 256; // most values between layers: four operands of 64
 
 struct MlpLayer {
     const uint8_t *codes, *scales;
@@ -669,43 +689,32 @@ __device__ __forceinline__ uint32_t lane_here()
     return lane;
 }
 
-// One layer's 32 outputs of a tile for the wave's rows: acc = bias + sum.
+// A tile of 32 outputs of a layer for the wave's rows, bias + sum.
 template <int PAIRS>
-__device__ __forceinline__ void mlp_tile(const MlpLayer &l, const char *lds, uint32_t lane, uint32_t tile, const u32x4 h[MLP_R][4],
-                                         const uint32_t hs[MLP_R], f32x16 acc[MLP_R])
+__device__ __forceinline__ f32x16 mlp_tile(const MlpLayer &l, const char *lds, uint32_t lane, uint32_t tile,
+                                           const u32x4 h[4], uint32_t hs)
 {
-    const uint32_t g = lane >> 5;
-    const char *b = lds + l.at_bias + (tile * 32 + 4 * g) * 4;
-    f32x16 init;
+    const char *b = lds + l.at_bias + (tile * 32 + 4 * (lane >> 5)) * 4;
+    f32x16 acc;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         const f32x4 v = *reinterpret_cast<const f32x4 *>(b + q * 32);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            init[4 * q + i] = v[i];
+            acc[4 * q + i] = v[i];
     }
     const uint32_t ws = *reinterpret_cast<const uint32_t *>(lds + l.at_scales + (tile * 64 + lane) * 4);
     const char *w = lds + l.at + tile * PAIRS * 1024 + lane * 16;
-    i32x8 a[PAIRS];
-#pragma unroll
-    for (int p = 0; p < PAIRS; ++p) {
-        const u32x4 q = *reinterpret_cast<const u32x4 *>(w + p * 1024);
-        a[p] = i32x8{(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0};
-    }
-#pragma unroll
-    for (int m = 0; m < MLP_R; ++m) {
-        acc[m] = init;
 #define VT_MLP_STEP(p)                                                                                                 \
-    if constexpr (PAIRS > p) {                                                                                         \
-        const i32x8 v = {(int)h[m][p][0], (int)h[m][p][1], (int)h[m][p][2], (int)h[m][p][3], 0, 0, 0, 0};              \
-        acc[m] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[p], v, acc[m], 4, 4, p, (int)ws, p, (int)hs[m]);    \
-    }
-        VT_MLP_STEP(0)
-        VT_MLP_STEP(1)
-        VT_MLP_STEP(2)
-        VT_MLP_STEP(3)
+    if constexpr (PAIRS > p)                                                                                           \
+        acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(*reinterpret_cast<const u32x4 *>(w + p * 1024)), \
+                                                              operand(h[p]), acc, 4, 4, p, (int)ws, p, (int)hs);
+    VT_MLP_STEP(0)
+    VT_MLP_STEP(1)
+    VT_MLP_STEP(2)
+    VT_MLP_STEP(3)
 #undef VT_MLP_STEP
-    }
+    return acc;
 }
 
 // The largest of 16 outputs and 0; NaN stays.
@@ -754,36 +763,27 @@ __device__ __forceinline__ u32x4 mlp_operand(const f32x16 &a, const f32x16 &b, u
 }
 
 template <int PAIRS, int TO>
-__device__ __forceinline__ void mlp_hidden(const MlpLayer &l, const char *lds, u32x4 h[MLP_R][4], uint32_t hs[MLP_R])
+__device__ __forceinline__ void mlp_hidden(const MlpLayer &l, const char *lds, u32x4 h[4], uint32_t &hs)
 {
     const uint32_t lane = lane_here();
-    u32x4 to[MLP_R][TO];
-    uint32_t to_s[MLP_R] = {};
+    u32x4 to[TO];
+    uint32_t to_s = 0;
 #pragma unroll
     for (int q = 0; q < TO; ++q) {
-        f32x16 acc[2][MLP_R];
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            mlp_tile<PAIRS>(l, lds, lane, 2 * q + b, h, hs, acc[b]);
-        }
-#pragma unroll
-        for (int m = 0; m < MLP_R; ++m) {
-            uint32_t c;
-            to[m][q] = mlp_operand(acc[0][m], acc[1][m], c);
-            to_s[m] |= c << (8 * q);
-        }
+        const f32x16 a = mlp_tile<PAIRS>(l, lds, lane, 2 * q, h, hs);
+        const f32x16 b = mlp_tile<PAIRS>(l, lds, lane, 2 * q + 1, h, hs);
+        uint32_t c;
+        to[q] = mlp_operand(a, b, c);
+        to_s |= c << (8 * q);
     }
 #pragma unroll
-    for (int m = 0; m < MLP_R; ++m) {
-#pragma unroll
-        for (int q = 0; q < TO; ++q)
-            h[m][q] = to[m][q];
-        hs[m] = to_s[m];
-    }
+    for (int q = 0; q < TO; ++q)
+        h[q] = to[q];
+    hs = to_s;
 }
 
 template <int PAIRS>
-__device__ __forceinline__ void mlp_hidden(const MlpLayer &l, const char *lds, u32x4 h[MLP_R][4], uint32_t hs[MLP_R])
+__device__ __forceinline__ void mlp_hidden(const MlpLayer &l, const char *lds, u32x4 h[4], uint32_t &hs)
 {
     switch (mlp_pairs(l.out)) {
     case 1: mlp_hidden<PAIRS, 1>(l, lds, h, hs); break;
@@ -793,7 +793,7 @@ __device__ __forceinline__ void mlp_hidden(const MlpLayer &l, const char *lds, u
     }
 }
 
-__device__ __forceinline__ void mlp_layer(const MlpLayer &l, const char *lds, u32x4 h[MLP_R][4], uint32_t hs[MLP_R])
+__device__ __forceinline__ void mlp_layer(const MlpLayer &l, const char *lds, u32x4 h[4], uint32_t &hs)
 {
     switch (mlp_pairs(l.width)) {
     case 1: mlp_hidden<1>(l, lds, h, hs); break;
@@ -804,64 +804,33 @@ __device__ __forceinline__ void mlp_layer(const MlpLayer &l, const char *lds, u3
 }
 
 template <int PAIRS, typename Y>
-__device__ __forceinline__ void mlp_last(const MlpLayer &l, const char *lds, const u32x4 h[MLP_R][4],
-                                         const uint32_t hs[MLP_R], uint64_t m0, uint64_t rows, Y *y)
+__device__ __forceinline__ void mlp_last(const MlpLayer &l, const char *lds, const u32x4 h[4], uint32_t hs, uint64_t m0,
+                                         uint64_t rows, Y *y)
 {
-    const uint32_t lane = lane_here(), r = lane & 31, g = lane >> 5;
+    const uint32_t lane = lane_here();
+    const uint64_t row = m0 + (lane & 31);
     for (uint32_t t = 0; t * 32 < l.out; ++t) {
-        f32x16 acc[MLP_R];
-        mlp_tile<PAIRS>(l, lds, lane, t, h, hs, acc);
+        const f32x16 acc = mlp_tile<PAIRS>(l, lds, lane, t, h, hs);
 #pragma unroll
-        for (int m = 0; m < MLP_R; ++m) {
-            const uint64_t row = m0 + 32 * m + r;
-            // the halves trade runs of four, so that each has eight neighbouring outputs: 16 q + 8 g
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                float v[8];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float a0 = acc[m][8 * q + i], a1 = acc[m][8 * q + 4 + i];
-                    const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a0),
-                                                                    __builtin_bit_cast(uint32_t, a1), false, false);
-                    v[i] = __builtin_bit_cast(float, (uint32_t)s[0]);
-                    v[4 + i] = __builtin_bit_cast(float, (uint32_t)s[1]);
-                }
-                const uint32_t n = t * 32 + 16 * q + 8 * g;
-                if (row < rows && n < l.out)
-                    store_upto8(y + row * l.out + n, l.out - n, v);
-            }
+        for (int q = 0; q < 2; ++q) {
+            float v[8];
+            eight_outputs(acc, q, v);
+            const uint32_t n = t * 32 + 16 * q + 8 * (lane >> 5);
+            if (row < rows && n < l.out)
+                store_upto8(y + row * l.out + n, l.out - n, v);
         }
     }
 }
 
-// Rows of x as operands: a lane's block of 32 of row r, quantised.
+// Block 2 pair + lane / 32 of the row m0 + lane % 32, as it lies in memory.
 template <typename T>
-__device__ __forceinline__ void mlp_load(const T *x, int64_t x_stride, uint64_t m0, uint64_t rows, uint32_t width,
-                                         uint32_t pair, Mx4Piece<T> v[MLP_R][4])
+__device__ __forceinline__ void mlp_load(const MlpArgs &p, uint64_t m0, uint32_t pair, Mx4Piece<T> v[4])
 {
-    const uint32_t r = threadIdx.x & 31, k = 64 * pair + (threadIdx.x & 32), left = k < width ? width - k : 0;
+    const uint32_t k = 64 * pair + (threadIdx.x & 32), width = p.layer[0].width, left = k < width ? width - k : 0;
+    const T *at = (const T *)p.x + (int64_t)min(m0 + (threadIdx.x & 31), p.rows - 1) * p.x_stride + k;
 #pragma unroll
-    for (int m = 0; m < MLP_R; ++m) {
-        const T *at = x + (int64_t)min(m0 + 32 * m + r, rows - 1) * x_stride + k;
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i)
-            v[m][i].load(at + 8 * i, left > 8 * i ? left - 8 * i : 0);
-    }
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t mlp_quantize(const Mx4Piece<T> v[4], u32x4 &h)
-{
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        v[i].top(top);
-    const uint32_t c = mx4_scale(Mx4Piece<T>::top_bits(top));
-    const float scale = e8m0_value(c);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        h[i] = v[i].word(scale);
-    return c;
+    for (uint32_t i = 0; i < 4; ++i)
+        v[i].load(at + 8 * i, left > 8 * i ? left - 8 * i : 0);
 }
 
 template <typename T, typename Y>
@@ -873,47 +842,35 @@ __global__ __launch_bounds__(MLP_THREADS) void mx4_mlp_kernel(MlpArgs p)
     __syncthreads();
     // Tiles of rows to blocks in turn, so that few of them spread over the chip. The first 64 values of the next
     // tile's rows are on their way while this one's are in the first layer, and wait as codes.
-    const uint64_t step = (uint64_t)gridDim.x * (MLP_THREADS / 64) * (32 * MLP_R);
-    uint64_t m0 = (blockIdx.x + (uint64_t)(threadIdx.x / 64) * gridDim.x) * (32 * MLP_R);
-    const uint32_t width = p.layer[0].width, pairs = mlp_pairs(width);
-    const T *x = (const T *)p.x;
-    u32x4 first[MLP_R];
-    uint32_t first_s[MLP_R];
-    Mx4Piece<T> next[MLP_R][4];
-    auto turn = [&] { // the rows that have arrived, to codes
-#pragma unroll
-        for (int m = 0; m < MLP_R; ++m)
-            first_s[m] = mlp_quantize<T>(next[m], first[m]);
-    };
+    const uint64_t step = (uint64_t)gridDim.x * (MLP_THREADS / 64) * 32;
+    uint64_t m0 = (blockIdx.x + (uint64_t)(threadIdx.x / 64) * gridDim.x) * 32;
+    const uint32_t pairs = mlp_pairs(p.layer[0].width);
+    u32x4 first;
+    uint32_t first_s;
+    Mx4Piece<T> next[4];
     if (m0 < p.rows) {
-        mlp_load(x, p.x_stride, m0, p.rows, width, 0, next);
-        turn();
+        mlp_load<T>(p, m0, 0, next);
+        first_s = quantize_block(next, first);
     }
     for (; m0 < p.rows; m0 += step) {
-        u32x4 h[MLP_R][4];
-        uint32_t hs[MLP_R];
-#pragma unroll
-        for (int m = 0; m < MLP_R; ++m) {
-            h[m][0] = first[m];
-            hs[m] = first_s[m];
-        }
+        u32x4 h[4];
+        h[0] = first;
+        uint32_t hs = first_s;
 #pragma unroll
         for (uint32_t q = 1; q < 4; ++q) {
             if (q < pairs) {
-                Mx4Piece<T> v[MLP_R][4];
-                mlp_load(x, p.x_stride, m0, p.rows, width, q, v);
-#pragma unroll
-                for (int m = 0; m < MLP_R; ++m)
-                    hs[m] |= mlp_quantize<T>(v[m], h[m][q]) << (8 * q);
+                Mx4Piece<T> v[4];
+                mlp_load<T>(p, m0, q, v);
+                hs |= quantize_block(v, h[q]) << (8 * q);
             }
         }
         const bool more = m0 + step < p.rows;
         if (more)
-            mlp_load(x, p.x_stride, m0 + step, p.rows, width, 0, next);
+            mlp_load<T>(p, m0 + step, 0, next);
         if (p.layers > 1)
             mlp_layer(p.layer[0], lds, h, hs);
         if (more)
-            turn();
+            first_s = quantize_block(next, first);
         for (uint32_t i = 1; i + 1 < p.layers; ++i)
             mlp_layer(p.layer[i], lds, h, hs);
         const MlpLayer &l = p.layer[p.layers - 1];
@@ -949,11 +906,12 @@ static uint32_t mlp_places(const vt_mx4_layer *layers, uint32_t num_layers, MlpL
 
 static int launch_mlp(int x_dtype, int y_dtype, const MlpArgs &p, uint32_t lds, hipStream_t s)
 {
-    const uint64_t tiles = (p.rows + 32 * MLP_R - 1) / (32 * MLP_R);
+    const uint64_t tiles = (p.rows + 31) / 32;
     const uint32_t grid = (uint32_t)(tiles < 256 ? tiles : 256); // one block a CU
     return with_type(x_dtype, [&](auto t) -> int {
         return with_type(y_dtype, [&](auto u) -> int {
-            auto kernel = mx4_mlp_kernel<decltype(t), decltype(u)>;
+            typedef decltype(t) T;
+            auto kernel = mx4_mlp_kernel<T, decltype(u)>;
             if (lds > 65536)
                 VT_HIP_CHECK(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
                                                  (int)MLP_LDS));
