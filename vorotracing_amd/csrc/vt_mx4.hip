@@ -387,138 +387,117 @@ __global__ __launch_bounds__(STREAM_THREADS, (stream_blocks<T, PAIRS> * 2)) void
     }
 }
 
-// Any size, both operands stored: a block's tile of 64 WM rows by 32 NT WN
-// outputs, each wave 64 rows by 32 NT outputs of it.  256 inputs (8 blocks) of
-// both sides at a time go straight into shared memory
-// (global_load_lds_dwordx4), the next ones while these are multiplied.  Bound
-// by the matrix products; 16 rows of 128 bytes are read from shared memory at
-// once, so the eight blocks of a row lie in an order of their own, by (row / 2).
+// Any size, both operands stored: a block of four waves takes a tile of 128
+// rows by 128 outputs, each wave 64 by 64.  256 inputs (8 blocks) of both sides
+// at a time go straight into shared memory (global_load_lds_dwordx4), the next
+// ones while these are multiplied.  16 rows of 128 bytes are read from shared
+// memory at once, so the blocks of a row lie in an order of their own, turned
+// by (row / 2), which no two of the 16 share within a bank.
+//
+// Larger tiles (256 by 256, eight waves of 64 by 128) would halve the reads of
+// shared memory but keep 128 registers of sums a lane, and spilled the rest
+// (16,384 by 2,048 by 2,048: 180 us against 71).
+constexpr uint32_t TILE = 128, TILE_THREADS = 256, TILE_WAVES = TILE_THREADS / 64;
 constexpr uint32_t TILE_BLOCKS = 8, TILE_ROW = 16 * TILE_BLOCKS;
+constexpr uint32_t TILE_LOAD_ROWS = 1024 / TILE_ROW; // that one load of a wave brings
+constexpr uint32_t TILE_LOADS = TILE / TILE_LOAD_ROWS / TILE_WAVES;
+constexpr uint32_t TILE_AT_W = TILE * TILE_ROW, TILE_AT_SCALES = 2 * TILE_AT_W;
+constexpr uint32_t TILE_STAGE = TILE_AT_SCALES + 2 * TILE * TILE_BLOCKS;
+static_assert(TILE_WAVES * OUT_BYTES <= 2 * TILE_STAGE, "the waves' places for y reuse the stages");
 
-template <int WM, int WN, int NT>
-struct TileShape {
-    static constexpr uint32_t M = 64 * WM, N = 32 * NT * WN, WAVES = WM * WN, THREADS = 64 * WAVES;
-    static constexpr uint32_t STAGE = (M + N) * (TILE_ROW + TILE_BLOCKS); // codes of both, then scales of both
-    static constexpr uint32_t LDS = 2 * STAGE;
-    static_assert(WAVES * OUT_BYTES <= LDS, "the waves' places for y reuse the stages");
-};
+// How the blocks of a row are turned.
+__device__ __forceinline__ uint32_t tile_turn(uint32_t row) { return row / (16 / TILE_BLOCKS) & (TILE_BLOCKS - 1); }
 
-// One side's rows row0 .. row0 + ROWS - 1 (the last row again past the end).
-template <uint32_t ROWS, uint32_t WAVES>
+// One side's 128 rows from row0 on (the last row again past the end).
 struct TileSide {
-    static constexpr uint32_t LOADS = ROWS / 8 / WAVES, SCALES = (ROWS + 64 * WAVES - 1) / (64 * WAVES);
-    static_assert(WAVES % 2 == 0, "a lane's place in the order of blocks is the same in all of its loads");
-    const uint8_t *codes, *scales; // of row0
-    uint32_t blocks, at[LOADS], at_scales[SCALES], place;
-    u32x2 c[SCALES];
+    const uint8_t *codes; // of row0
+    uint32_t blocks, at[TILE_LOADS], place;
 
-    __device__ __forceinline__ void begin(const uint8_t *x, const uint8_t *xs, uint64_t row0, uint64_t rows,
-                                          uint32_t blocks_)
+    __device__ __forceinline__ void begin(const uint8_t *x, uint64_t row0, uint64_t rows, uint32_t blocks_)
     {
-        const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, last = (uint32_t)min(rows - 1 - row0, (uint64_t)ROWS);
+        const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, last = (uint32_t)min(rows - 1 - row0, (uint64_t)TILE);
         blocks = blocks_;
         codes = x + row0 * blocks * 16;
-        scales = xs + row0 * blocks;
-        place = (lane & 7) ^ (4 * (wave & 1) | lane / 16); // row / 2 % 8
+        // the rows of a lane's loads are 32 or 64 apart and turn alike
+        place = (lane & (TILE_BLOCKS - 1)) ^ tile_turn(wave * TILE_LOAD_ROWS + lane / TILE_BLOCKS);
 #pragma unroll
-        for (uint32_t i = 0; i < LOADS; ++i)
-            at[i] = min((i * WAVES + wave) * 8 + lane / 8, last) * blocks * 16 + place * 16;
-#pragma unroll
-        for (uint32_t i = 0; i < SCALES; ++i)
-            at_scales[i] = min(i * 64 * WAVES + threadIdx.x, last) * blocks;
+        for (uint32_t i = 0; i < TILE_LOADS; ++i)
+            at[i] = min((i * TILE_WAVES + wave) * TILE_LOAD_ROWS + lane / TILE_BLOCKS, last) * blocks * 16 + place * 16;
     }
 
-    // blocks j0 .. j0 + 7, all within the rows: codes to shared memory, scales to registers
-    __device__ __forceinline__ void bring(uint32_t j0, char *to)
+    // blocks from j0 on, all within the rows, to shared memory
+    __device__ __forceinline__ void bring(uint32_t j0, char *to) const
     {
         const uint32_t wave = threadIdx.x >> 6;
         // one base for all lanes, and not a pointer of its own for each load
-        j0 = __builtin_amdgcn_readfirstlane(j0);
-        const uint8_t *x = codes + j0 * 16, *xs = scales + j0;
+        const uint8_t *x = codes + __builtin_amdgcn_readfirstlane(j0) * 16;
 #pragma unroll
-        for (uint32_t i = 0; i < LOADS; ++i)
+        for (uint32_t i = 0; i < TILE_LOADS; ++i)
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(x + at[i]),
-                                             (__attribute__((address_space(3))) void *)(to + (i * WAVES + wave) * 1024),
+                                             (__attribute__((address_space(3))) void *)(to + (i * TILE_WAVES + wave) * 1024),
                                              16, 0, 0);
-#pragma unroll
-        for (uint32_t i = 0; i < SCALES; ++i)
-            c[i] = *reinterpret_cast<const u32x2_any *>(xs + at_scales[i]);
     }
 
-    // the rows' last blocks from j0 on, fewer than 8, and zeros behind them
-    __device__ __forceinline__ void bring_last(uint32_t j0, char *to)
+    // the rows' last blocks from j0 on and zeros behind them
+    __device__ __forceinline__ void bring_last(uint32_t j0, char *to) const
     {
         const uint32_t wave = threadIdx.x >> 6;
 #pragma unroll
-        for (uint32_t i = 0; i < LOADS; ++i) {
+        for (uint32_t i = 0; i < TILE_LOADS; ++i) {
             u32x4 q = {};
             if (j0 + place < blocks)
                 q = *reinterpret_cast<const u32x4_any *>(codes + j0 * 16 + at[i]);
-            *reinterpret_cast<u32x4 *>(to + (i * WAVES + wave) * 1024 + (threadIdx.x & 63) * 16) = q;
+            *reinterpret_cast<u32x4 *>(to + (i * TILE_WAVES + wave) * 1024 + (threadIdx.x & 63) * 16) = q;
         }
-#pragma unroll
-        for (uint32_t i = 0; i < SCALES; ++i) {
-            uint64_t v = 0x7f7f7f7f7f7f7f7full;
-#pragma unroll 1
-            for (uint32_t j = 0; j < blocks - j0; ++j)
-                v = (v & ~(255ull << (8 * j))) | (uint64_t)scales[at_scales[i] + j0 + j] << (8 * j);
-            c[i] = __builtin_bit_cast(u32x2, v);
-        }
-    }
-
-    __device__ __forceinline__ void put_scales(char *to) const
-    {
-#pragma unroll
-        for (uint32_t i = 0; i < SCALES; ++i)
-            if (i * 64 * WAVES + threadIdx.x < ROWS)
-                *reinterpret_cast<u32x2 *>(to + (i * 64 * WAVES + threadIdx.x) * 8) = c[i];
     }
 };
 
-template <int WM, int WN, int NT>
-__global__ __launch_bounds__(64 * WM *WN, 2) void mx4_tile_kernel(LinearArgs p)
+__global__ __launch_bounds__(TILE_THREADS, 2) void mx4_tile_kernel(LinearArgs p)
 {
-    typedef TileShape<WM, WN, NT> S;
+    typedef uint32_t scales_t __attribute__((ext_vector_type(TILE_BLOCKS / 4)));
+    typedef uint32_t scales_any __attribute__((ext_vector_type(TILE_BLOCKS / 4), aligned(1)));
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const uint32_t tiles_n = (p.out + S::N - 1) / S::N, blocks = mx_blocks(p.width);
+    const uint32_t tiles_n = (p.out + TILE - 1) / TILE, blocks = mx_blocks(p.width);
     // Blocks go to the 8 dies in turn: one die takes all outputs of a range of rows.
     const uint32_t slot = blockIdx.x / 8;
-    const uint64_t m0 = (uint64_t)(slot / tiles_n * 8 + blockIdx.x % 8) * S::M;
-    const uint32_t n0 = slot % tiles_n * S::N;
+    const uint64_t m0 = (uint64_t)(slot / tiles_n * 8 + blockIdx.x % 8) * TILE;
+    const uint32_t n0 = slot % tiles_n * TILE;
     if (m0 >= p.rows)
         return;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, g = lane >> 5;
-    const uint32_t wm = wave / WN * 64, wn = wave % WN * (32 * NT);
+    const uint32_t wm = wave / 2 * 64, wn = wave % 2 * 64;
 
-    TileSide<S::M, S::WAVES> x;
-    TileSide<S::N, S::WAVES> w;
-    x.begin((const uint8_t *)p.x, p.xs, m0, p.rows, blocks);
-    w.begin(p.w, p.ws, n0, p.out, blocks);
-    constexpr uint32_t AT_W = S::M * TILE_ROW, AT_XS = AT_W + S::N * TILE_ROW, AT_WS = AT_XS + S::M * 8;
+    TileSide x, w;
+    x.begin((const uint8_t *)p.x, m0, p.rows, blocks);
+    w.begin(p.w, n0, p.out, blocks);
+    // half of the threads bring the scales of a row of x each, half of w
+    const uint8_t *scales_of = threadIdx.x < TILE ? p.xs + min(m0 + threadIdx.x, p.rows - 1) * blocks
+                                                  : p.ws + (uint64_t)min(n0 + threadIdx.x - TILE, p.out - 1) * blocks;
+    const uint32_t scales_at = TILE_AT_SCALES + threadIdx.x * TILE_BLOCKS;
     // codes that go straight into shared memory count as loads of the wave that asked for them
     auto arrived = [] {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
     };
-    f32x16 acc[NT][2] = {};
-    const uint32_t turn = r >> 1 & 7; // rows 32 apart turn alike
+    f32x16 acc[2][2] = {};
+    const uint32_t turn = tile_turn(r); // rows 32 apart turn alike
     auto products = [&](const char *stage) {
         // a lane's scales: its rows' words, of which bytes 0 and 2 are for the blocks g and 2 + g
-        u32x2 ca[2], cb[NT];
+        scales_t ca[2], cb[2];
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
-            ca[m] = *reinterpret_cast<const u32x2 *>(stage + AT_XS + (wm + 32 * m + r) * 8) >> (8 * g);
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-            cb[n] = *reinterpret_cast<const u32x2 *>(stage + AT_WS + (wn + 32 * n + r) * 8) >> (8 * g);
-        const char *xa = stage + (wm + r) * TILE_ROW, *wa = stage + AT_W + (wn + r) * TILE_ROW;
+        for (int m = 0; m < 2; ++m) {
+            ca[m] = *reinterpret_cast<const scales_t *>(stage + TILE_AT_SCALES + (wm + 32 * m + r) * TILE_BLOCKS) >> (8 * g);
+            cb[m] = *reinterpret_cast<const scales_t *>(stage + TILE_AT_SCALES + (TILE + wn + 32 * m + r) * TILE_BLOCKS) >>
+                    (8 * g);
+        }
+        const char *xa = stage + (wm + r) * TILE_ROW, *wa = stage + TILE_AT_W + (wn + r) * TILE_ROW;
 #define VT_TILE_STEP(q)                                                                                                \
-    {                                                                                                                  \
+    if constexpr (2 * q < TILE_BLOCKS) {                                                                               \
         const uint32_t at = ((2 * q + g) ^ turn) * 16;                                                                 \
         i32x8 v[2];                                                                                                    \
         _Pragma("unroll") for (int m = 0; m < 2; ++m) v[m] =                                                           \
             operand(*reinterpret_cast<const u32x4 *>(xa + m * 32 * TILE_ROW + at));                                    \
-        _Pragma("unroll") for (int n = 0; n < NT; ++n)                                                                 \
+        _Pragma("unroll") for (int n = 0; n < 2; ++n)                                                                  \
         {                                                                                                              \
             const i32x8 a = operand(*reinterpret_cast<const u32x4 *>(wa + n * 32 * TILE_ROW + at));                    \
             _Pragma("unroll") for (int m = 0; m < 2; ++m) acc[n][m] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4( \
@@ -533,19 +512,18 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void mx4_tile_kernel(LinearArgs p)
     };
     const uint32_t full = blocks / TILE_BLOCKS * TILE_BLOCKS;
     if (full) {
-        x.bring(0, lds);
-        w.bring(0, lds + AT_W);
-        x.put_scales(lds + AT_XS);
-        w.put_scales(lds + AT_WS);
+        char *stage = lds, *next = lds + TILE_STAGE;
+        x.bring(0, stage);
+        w.bring(0, stage + TILE_AT_W);
+        *reinterpret_cast<scales_t *>(stage + scales_at) = *reinterpret_cast<const scales_any *>(scales_of);
         arrived();
-        char *stage = lds, *next = lds + S::STAGE;
         for (uint32_t j0 = TILE_BLOCKS; j0 < full; j0 += TILE_BLOCKS) {
             x.bring(j0, next);
-            w.bring(j0, next + AT_W);
+            w.bring(j0, next + TILE_AT_W);
+            const scales_t c = *reinterpret_cast<const scales_any *>(scales_of + j0);
             products(stage);
             __builtin_amdgcn_sched_barrier(0); // the products do not wait for the next scales
-            x.put_scales(next + AT_XS);
-            w.put_scales(next + AT_WS);
+            *reinterpret_cast<scales_t *>(next + scales_at) = c;
             arrived(); // and this stage has been read
             char *t = stage;
             stage = next;
@@ -556,22 +534,22 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void mx4_tile_kernel(LinearArgs p)
     }
     if (full < blocks) {
         x.bring_last(full, lds);
-        w.bring_last(full, lds + AT_W);
-        x.put_scales(lds + AT_XS);
-        w.put_scales(lds + AT_WS);
+        w.bring_last(full, lds + TILE_AT_W);
+        for (uint32_t j = 0; j < TILE_BLOCKS; ++j)
+            lds[scales_at + j] = full + j < blocks ? scales_of[full + j] : 127;
         __syncthreads();
         products(lds);
         __syncthreads();
     }
     char *place = lds + wave * OUT_BYTES;
-    const uint32_t nw = n0 + wn, left = nw < p.out ? p.out - nw : 0, tiles = min((left + 31) / 32, (uint32_t)NT);
+    const uint32_t nw = n0 + wn, left = nw < p.out ? p.out - nw : 0, tiles = min((left + 31) / 32, 2u);
     auto put = [&](auto y) {
         typedef decltype(y) Y;
         constexpr uint32_t TILES = 4 / sizeof(Y); // of 32 outputs in 128 bytes
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
-            for (uint32_t t = 0; t < (uint32_t)NT; ++t) {
+            for (uint32_t t = 0; t < 2; ++t) {
                 if (t >= tiles)
                     continue;
                 stage_tile<Y>(place, t, acc[t][m], p.relu, p.bias, nw + 32 * t, p.out);
@@ -988,15 +966,16 @@ static int launch_rows(const LinearArgs &p, LinearForm form, hipStream_t s)
     }
 }
 
-template <int WM, int WN, int NT>
 static int launch_tiles(const LinearArgs &p, hipStream_t s)
 {
-    typedef TileShape<WM, WN, NT> S;
-    const uint64_t grid = ((p.rows + S::M - 1) / S::M + 7) / 8 * 8 * ((p.out + S::N - 1) / S::N);
+    const uint64_t grid = ((p.rows + TILE - 1) / TILE + 7) / 8 * 8 * ((p.out + TILE - 1) / TILE);
     VT_REQUIRE(grid < (1ull << 31), "%llu rows by %u outputs are too many for one call", (unsigned long long)p.rows, p.out);
-    auto kernel = mx4_tile_kernel<WM, WN, NT>;
-    VT_HIP_CHECK(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::LDS));
-    kernel<<<(uint32_t)grid, S::THREADS, S::LDS, s>>>(p);
+    // a lane's place among a tile's codes is a 32-bit offset
+    VT_REQUIRE(p.width < (1u << 25), "%u inputs are too many for one call", p.width);
+    constexpr int LDS = 2 * TILE_STAGE;
+    if (LDS > 65536)
+        VT_HIP_CHECK(hipFuncSetAttribute((const void *)mx4_tile_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+    mx4_tile_kernel<<<(uint32_t)grid, TILE_THREADS, LDS, s>>>(p);
     VT_LAUNCH_CHECK("mx4_tile_kernel");
     return VT_OK;
 }
@@ -1021,7 +1000,7 @@ static int linear(int x_dtype, LinearArgs p, void *workspace, hipStream_t s)
         p.x = codes;
         p.xs = scales;
     }
-    return launch_tiles<2, 2, 2>(p, s);
+    return launch_tiles(p, s);
 }
 
 } // namespace vt
