@@ -108,7 +108,8 @@ def _linear_want(x, w, bias, relu):
 
 LINEAR = [(1, 1, 1), (1, 512, 768), (1, 33, 1000), (2, 64, 16), (13, 100, 33), (16, 2048, 64), (17, 256, 256), (31, 31, 31),
           (33, 65, 130), (64, 128, 48), (100, 1000, 7), (130, 256, 256), (257, 333, 520), (300, 64, 300), (1000, 96, 1),
-          (2050, 512, 40), (0, 64, 8), (5, 64, 0), (5, 0, 3)]
+          (2050, 512, 40), (0, 64, 8), (5, 64, 0), (5, 0, 3), (40, 0, 3), (70, 2049, 200), (200, 600, 300), (150, 513, 128),
+          (33, 7000, 5)]
 
 
 @pytest.mark.parametrize("size", LINEAR)
@@ -186,6 +187,59 @@ def test_mlp_is_its_layers_in_turn(gpu):
     want = micro.linear_mx4(h, *layers[1])
     assert torch.equal(got.isnan(), want.isnan()) and bool(got[69000].isnan().all())
     assert torch.equal(got.nan_to_num(), want.nan_to_num()) and int(got.isnan().any(1).sum()) == 1
+
+
+def test_many_rows_go_round(gpu):
+    """More rows than the blocks of the product and of the head take at once."""
+    x = _rows((140001, 40), F16, 27, gpu)
+    w, bias = _weights(9, 40, 28, gpu)
+    for arg in (x, micro.quantize_mx4(x)):
+        got = micro.linear_mx4(arg, w, bias, dtype=F32)
+        want, s = _linear_want(O.mx4(O.f64(x))[2], O.f64(w.dequantize()), O.f64(bias), False)
+        _within(got, want, 42 * 2.0 ** -23 * s + O.rounding(want, F32))
+    layers = _exact_layers([40, 70, 33, 9], 29, gpu)
+    for dtype in TYPES:
+        y = (x.float() / 64).to(dtype)
+        got = micro.mlp_mx4(y, layers, dtype=F32)
+        h = y
+        for i, (weight, b) in enumerate(layers):
+            h = micro.linear_mx4(h, weight, b, relu=i < 2, dtype=F32)
+        assert torch.equal(got, h)
+
+
+def test_offsets_past_32_bits(gpu):
+    """Tensors of more than 2^32 values: their last rows are those of a call on them alone."""
+    x = torch.randn(5_000_000, 1024, device=gpu, dtype=BF16)
+    end = x[-100:].clone()
+    q, want = micro.quantize_mx4(x), micro.quantize_mx4(end)
+    assert torch.equal(q.codes[-100:], want.codes) and torch.equal(q.scales[-100:], want.scales)
+    back = q.dequantize(BF16)
+    assert torch.equal(back[-100:], want.dequantize(BF16))
+    del back
+    w, bias = _weights(3, 1024, 33, gpu)
+    got = micro.linear_mx4(q, w, bias)  # codes of 2.6 GB
+    assert torch.equal(got[-100:], micro.linear_mx4(want, w, bias))
+    del q, got
+    y, kept = micro.checkpoint_activation(x, "relu")
+    want_y, want_kept = micro.checkpoint_activation(end, "relu")
+    assert torch.equal(y[-100:], want_y) and torch.equal(kept.codes[-100:], want_kept.codes)
+    del y
+    dz = kept.input_grad(x)
+    assert torch.equal(dz[-100:], want_kept.input_grad(end))
+    del dz, x
+    dy = torch.zeros(5_000_000, 2, device=gpu, dtype=BF16)
+    dy[-64:] = 1
+    dw, db = kept.weight_grad(dy)
+    last = kept.dequantize(BF16)[-64:].float().clamp(min=0).double()
+    assert torch.allclose(dw.double(), last.sum(0).expand(2, -1), rtol=1e-5, atol=1e-5) and db.tolist() == [64.0, 64.0]
+    del kept
+    x = torch.randn(70_000_000, 1, device=gpu, dtype=F16)
+    w, bias = _weights(64, 1, 31, gpu)
+    y = micro.linear_mx4(x, w, bias)
+    assert torch.equal(y[-100:], micro.linear_mx4(x[-100:], w, bias))
+    layers = _exact_layers([1, 32, 64], 32, gpu)
+    y = micro.mlp_mx4(x, layers)
+    assert torch.equal(y[-100:], micro.mlp_mx4(x[-100:], layers))
 
 
 @pytest.mark.parametrize("act", ACTS)
