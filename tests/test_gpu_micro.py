@@ -177,6 +177,23 @@ def test_mlp(gpu, rows, widths, dtype, to):
     _within(got, h, (layers[-1][0].width + 2) * 2.0 ** -23 * s + O.rounding(h, to), widths)
 
 
+@pytest.mark.parametrize("rows,widths", [(3000, [40, 70, 33, 9]), (777, [256, 256, 256, 64]), (30, [60, 128, 128, 33])])
+def test_mlp_rounds_as_its_layers_do(gpu, rows, widths):
+    """Biases of all bits: the sums of one layer's 4-bit products are exact in f32, the bias is their one rounding in
+    every form of the product, and so the head's hidden values, scales and results are the layers', bit for bit."""
+    g = torch.Generator().manual_seed(34)
+    layers = [(micro.quantize_mx4((torch.randn(b, a, generator=g) / a ** 0.5).to(gpu)),
+               (0.1 * torch.randn(b, generator=g)).to(gpu)) for a, b in zip(widths, widths[1:])]
+    x = torch.randn(rows, widths[0], generator=g).to(gpu)
+    h = x
+    for i, (w, b) in enumerate(layers):
+        q, v = O.mx4(O.f64(h))[2], O.f64(w.dequantize())
+        h = micro.linear_mx4(h, w, b, relu=i + 1 < len(layers))
+        want = (q @ v.T).astype(np.float32) + O.f64(b).astype(np.float32)
+        assert np.array_equal(O.f64(h), np.maximum(want, 0) if i + 1 < len(layers) else want)
+    assert torch.equal(micro.mlp_mx4(x, layers), h)
+
+
 def test_mlp_is_its_layers_in_turn(gpu):
     """More rows than one pass over the workspace, and a NaN row that stays alone."""
     layers = _exact_layers([16, 288, 8], 9, gpu)

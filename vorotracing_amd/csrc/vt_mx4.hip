@@ -167,7 +167,7 @@ constexpr uint32_t OUT_PITCH = 144, OUT_BYTES = 32 * OUT_PITCH; // a wave's plac
 
 template <typename Y>
 __device__ __forceinline__ void stage_tile(char *place, uint32_t tile, const f32x16 &acc, int relu,
-                                           const float *bias = nullptr, uint32_t n0 = 0, uint32_t out = 0)
+                                           const float *bias, uint32_t n0, uint32_t out)
 {
     constexpr uint32_t PER = 128 / sizeof(Y); // outputs of a row at a time
     const uint32_t r = threadIdx.x & 31, g = threadIdx.x >> 5 & 1;
@@ -229,11 +229,11 @@ __device__ __forceinline__ void wave_order()
 }
 
 template <typename Y>
-__device__ __forceinline__ void put_tile(char *place, uint32_t tile, uint32_t tiles, const f32x16 &acc, int relu, void *y,
-                                         uint64_t m0, uint64_t rows, uint32_t out)
+__device__ __forceinline__ void put_tile(char *place, uint32_t tile, uint32_t tiles, const f32x16 &acc, const float *bias,
+                                         int relu, void *y, uint64_t m0, uint64_t rows, uint32_t out)
 {
     constexpr uint32_t TILES = 4 / sizeof(Y); // of 32 outputs in 128 bytes
-    stage_tile<Y>(place, tile, acc, relu);
+    stage_tile<Y>(place, tile, acc, relu, bias, 32 * tile, (tile + 1) * 32);
     if (tile % TILES == TILES - 1 || tile + 1 == tiles) {
         wave_order();
         store_staged<Y>(place, (Y *)y, m0, rows, tile / TILES * TILES * 32, out);
@@ -353,15 +353,8 @@ __global__ __launch_bounds__(STREAM_THREADS, (stream_blocks<T, PAIRS> * 2)) void
             }
         }
         for (uint32_t t = 0; t < tiles; ++t) {
-            f32x16 acc;
-            const char *b = lds_b + (t * 32 + 4 * g) * 4, *w = lds + (t * PAIRS * 64 + lane) * 16;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const f32x4 v = *reinterpret_cast<const f32x4 *>(b + q * 32);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    acc[4 * q + i] = v[i];
-            }
+            f32x16 acc = {};
+            const char *w = lds + (t * PAIRS * 64 + lane) * 16;
             const u32x2 s = *reinterpret_cast<const u32x2 *>(lds_s + (t * 64 + lane) * 8);
 #define VT_STREAM_STEP(q)                                                                                              \
     if constexpr (PAIRS > q)                                                                                           \
@@ -377,12 +370,13 @@ __global__ __launch_bounds__(STREAM_THREADS, (stream_blocks<T, PAIRS> * 2)) void
             VT_STREAM_STEP(6)
             VT_STREAM_STEP(7)
 #undef VT_STREAM_STEP
+            const float *bias = reinterpret_cast<const float *>(lds_b);
             if (p.y_dtype == VT_F32)
-                put_tile<float>(place, t, tiles, acc, p.relu, p.y, m0, p.rows, p.out);
+                put_tile<float>(place, t, tiles, acc, bias, p.relu, p.y, m0, p.rows, p.out);
             else if (p.y_dtype == VT_F16)
-                put_tile<_Float16>(place, t, tiles, acc, p.relu, p.y, m0, p.rows, p.out);
+                put_tile<_Float16>(place, t, tiles, acc, bias, p.relu, p.y, m0, p.rows, p.out);
             else
-                put_tile<__bf16>(place, t, tiles, acc, p.relu, p.y, m0, p.rows, p.out);
+                put_tile<__bf16>(place, t, tiles, acc, bias, p.relu, p.y, m0, p.rows, p.out);
         }
     }
 }
@@ -672,15 +666,7 @@ template <int PAIRS>
 __device__ __forceinline__ f32x16 mlp_tile(const MlpLayer &l, const char *lds, uint32_t lane, uint32_t tile,
                                            const u32x4 h[4], uint32_t hs)
 {
-    const char *b = lds + l.at_bias + (tile * 32 + 4 * (lane >> 5)) * 4;
-    f32x16 acc;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const f32x4 v = *reinterpret_cast<const f32x4 *>(b + q * 32);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            acc[4 * q + i] = v[i];
-    }
+    f32x16 acc = {};
     const uint32_t ws = *reinterpret_cast<const uint32_t *>(lds + l.at_scales + (tile * 64 + lane) * 4);
     const char *w = lds + l.at + tile * PAIRS * 1024 + lane * 16;
 #define VT_MLP_STEP(p)                                                                                                 \
@@ -692,7 +678,12 @@ __device__ __forceinline__ f32x16 mlp_tile(const MlpLayer &l, const char *lds, u
     VT_MLP_STEP(2)
     VT_MLP_STEP(3)
 #undef VT_MLP_STEP
-    return acc;
+    // Sums of e2m1 products are exact in f32 while the blocks' scales lie within some powers of two of each other, and the
+    // bias behind them is then the one rounding, whatever the order: as the first summand it would round at every step,
+    // and a last bit at the edge of a power of two turns the next block's scale. The f32 product bias x 1 adds it to all
+    // rows (1 instruction and 1 read of shared memory, for 16 additions and 4 reads).
+    const float b = lane < 32 ? *reinterpret_cast<const float *>(lds + l.at_bias + (tile * 32 + (lane & 31)) * 4) : 0.0f;
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(b, 1.0f, acc, 0, 0, 0);
 }
 
 // The largest of 16 outputs and 0; NaN stays.
