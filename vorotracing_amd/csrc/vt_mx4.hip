@@ -146,6 +146,19 @@ __device__ __forceinline__ i32x8 operand(const u32x4 &q)
     return i32x8{(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0};
 }
 
+// A tile's sums and its outputs' biases, of which lane l brings that of output
+// l % 32.  Sums of e2m1 products are exact in f32 while the blocks' scales lie
+// within some powers of two of each other, and the bias behind them is then
+// the one rounding, whatever the order: as the first summand it would round at
+// every step, and a last bit at the edge of a power of two turns the scale of a
+// block that is made of the result.  The f32 product bias x 1 adds it to all
+// rows: 1 instruction and 1 read, for 16 additions and 4 reads.
+__device__ __forceinline__ f32x16 add_bias(const f32x16 &acc, float bias)
+{
+    const float lower = threadIdx.x & 32 ? 0.0f : bias; // the upper lanes are the product's second step
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(lower, 1.0f, acc, 0, 0, 0);
+}
+
 // Outputs 16 q + 8 (l / 32) .. + 7 of a lane's row, of its tile of 32: the
 // halves of the wave trade runs of four.
 __device__ __forceinline__ void eight_outputs(const f32x16 &acc, int q, float v[8])
@@ -166,8 +179,7 @@ __device__ __forceinline__ void eight_outputs(const f32x16 &acc, int q, float v[
 constexpr uint32_t OUT_PITCH = 144, OUT_BYTES = 32 * OUT_PITCH; // a wave's place
 
 template <typename Y>
-__device__ __forceinline__ void stage_tile(char *place, uint32_t tile, const f32x16 &acc, int relu,
-                                           const float *bias, uint32_t n0, uint32_t out)
+__device__ __forceinline__ void stage_tile(char *place, uint32_t tile, const f32x16 &acc, int relu)
 {
     constexpr uint32_t PER = 128 / sizeof(Y); // outputs of a row at a time
     const uint32_t r = threadIdx.x & 31, g = threadIdx.x >> 5 & 1;
@@ -175,14 +187,6 @@ __device__ __forceinline__ void stage_tile(char *place, uint32_t tile, const f32
     for (int q = 0; q < 2; ++q) {
         float v[8];
         eight_outputs(acc, q, v);
-        if (bias) {
-            const uint32_t n = n0 + 16 * q + 8 * g;
-            float b[8];
-            load_upto8(bias + n, n < out ? out - n : 0, b);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                v[i] += b[i];
-        }
         if (relu) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -229,11 +233,11 @@ __device__ __forceinline__ void wave_order()
 }
 
 template <typename Y>
-__device__ __forceinline__ void put_tile(char *place, uint32_t tile, uint32_t tiles, const f32x16 &acc, const float *bias,
-                                         int relu, void *y, uint64_t m0, uint64_t rows, uint32_t out)
+__device__ __forceinline__ void put_tile(char *place, uint32_t tile, uint32_t tiles, const f32x16 &acc, int relu, void *y,
+                                         uint64_t m0, uint64_t rows, uint32_t out)
 {
     constexpr uint32_t TILES = 4 / sizeof(Y); // of 32 outputs in 128 bytes
-    stage_tile<Y>(place, tile, acc, relu, bias, 32 * tile, (tile + 1) * 32);
+    stage_tile<Y>(place, tile, acc, relu);
     if (tile % TILES == TILES - 1 || tile + 1 == tiles) {
         wave_order();
         store_staged<Y>(place, (Y *)y, m0, rows, tile / TILES * TILES * 32, out);
@@ -370,13 +374,13 @@ __global__ __launch_bounds__(STREAM_THREADS, (stream_blocks<T, PAIRS> * 2)) void
             VT_STREAM_STEP(6)
             VT_STREAM_STEP(7)
 #undef VT_STREAM_STEP
-            const float *bias = reinterpret_cast<const float *>(lds_b);
+            acc = add_bias(acc, *reinterpret_cast<const float *>(lds_b + (t * 32 + r) * 4));
             if (p.y_dtype == VT_F32)
-                put_tile<float>(place, t, tiles, acc, bias, p.relu, p.y, m0, p.rows, p.out);
+                put_tile<float>(place, t, tiles, acc, p.relu, p.y, m0, p.rows, p.out);
             else if (p.y_dtype == VT_F16)
-                put_tile<_Float16>(place, t, tiles, acc, bias, p.relu, p.y, m0, p.rows, p.out);
+                put_tile<_Float16>(place, t, tiles, acc, p.relu, p.y, m0, p.rows, p.out);
             else
-                put_tile<__bf16>(place, t, tiles, acc, bias, p.relu, p.y, m0, p.rows, p.out);
+                put_tile<__bf16>(place, t, tiles, acc, p.relu, p.y, m0, p.rows, p.out);
         }
     }
 }
@@ -546,7 +550,8 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void mx4_tile_kernel(LinearArgs p)
             for (uint32_t t = 0; t < 2; ++t) {
                 if (t >= tiles)
                     continue;
-                stage_tile<Y>(place, t, acc[t][m], p.relu, p.bias, nw + 32 * t, p.out);
+                const uint32_t o = nw + 32 * t + r;
+                stage_tile<Y>(place, t, add_bias(acc[t][m], p.bias && o < p.out ? p.bias[o] : 0.0f), p.relu);
                 if (t % TILES == TILES - 1 || t + 1 == tiles) {
                     wave_order();
                     store_staged<Y>(place, (Y *)p.y, m0 + wm + 32 * m, p.rows, nw + t / TILES * TILES * 32, p.out);
@@ -678,12 +683,8 @@ __device__ __forceinline__ f32x16 mlp_tile(const MlpLayer &l, const char *lds, u
     VT_MLP_STEP(2)
     VT_MLP_STEP(3)
 #undef VT_MLP_STEP
-    // Sums of e2m1 products are exact in f32 while the blocks' scales lie within some powers of two of each other, and the
-    // bias behind them is then the one rounding, whatever the order: as the first summand it would round at every step,
-    // and a last bit at the edge of a power of two turns the next block's scale. The f32 product bias x 1 adds it to all
-    // rows (1 instruction and 1 read of shared memory, for 16 additions and 4 reads).
-    const float b = lane < 32 ? *reinterpret_cast<const float *>(lds + l.at_bias + (tile * 32 + (lane & 31)) * 4) : 0.0f;
-    return __builtin_amdgcn_mfma_f32_32x32x2f32(b, 1.0f, acc, 0, 0, 0);
+    const uint32_t n = tile * 32 + (lane & 31);
+    return add_bias(acc, *reinterpret_cast<const float *>(lds + l.at_bias + n * 4));
 }
 
 // The largest of 16 outputs and 0; NaN stays.
