@@ -109,7 +109,8 @@ __device__ __forceinline__ void load_codes(const uint8_t *p, uint32_t n, uint32_
 }
 
 // Eight values a thread, a block's four threads side by side, as the 4-bit
-// quantisation.
+// quantisation.  Bound by memory: 480,000 rows of 256 in bf16 with ReLU 101 us,
+// 6.1 TB/s (some of it from the cache behind the L2), the backward pass 113 us.
 template <typename T, int ACT>
 __global__ __launch_bounds__(ACT_THREADS) void act_checkpoint_kernel(const T *__restrict__ z, int64_t z_stride,
                                                                      uint64_t groups, uint32_t width, T *__restrict__ y,
@@ -200,6 +201,12 @@ __global__ __launch_bounds__(ACT_THREADS) void ckpt8_read_kernel(const uint8_t *
 // but the f32 sum.  A wider factor is split into bf16 parts that hold all of
 // its bits (f16: 2, f32 and the smooth activations: 3), and the products of
 // parts down to 2^-16 of the first are summed (2, 3, 5 or 6 instructions).
+//
+// Ranges of rows, three blocks a CU, keep the loads of two steps each on their
+// way; a second kernel joins them in their order, so that the same inputs give
+// the same bits.  Bound by memory and its latency: 480,000 rows, 256 by 256, bf16
+// 102 us + 9 to join, 4.1 TB/s with the ranges' sums (50 MB); 239 us before bf16
+// went to shared memory as it is and bank conflicts were turned away.
 constexpr int WG_THREADS = 256, WG_N = 128, WG_K = 128, WG_M = 32;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
