@@ -441,6 +441,10 @@ def test_refusals(gpu):
         micro.linear_mx4(x, w, dtype=torch.float64)
     with pytest.raises(ValueError, match="records no gradient"):
         micro.linear_mx4(x.clone().requires_grad_(), w)
+    with pytest.raises(ValueError, match="records no gradient"):
+        micro.mlp_mx4(x, [(w, bias.clone().requires_grad_())])
+    with torch.no_grad():
+        micro.linear_mx4(x.clone().requires_grad_(), w, bias.clone().requires_grad_())
     with pytest.raises(ValueError, match="1 to 16 layers"):
         micro.mlp_mx4(x, [])
     with pytest.raises(ValueError, match="8 values with weights of"):

@@ -173,6 +173,8 @@ def _check_layer(what: str, weight, bias, width: int, device):
     if bias is not None:
         if bias.dtype != torch.float32 or tuple(bias.shape) != (weight.codes.shape[0],) or not bias.is_contiguous():
             raise ValueError(f"{what}: the bias is a contiguous float32 tensor of {weight.codes.shape[0]}")
+        if bias.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{what}: this operator records no gradient; detach the bias")
     _same_device(what, device, weight.codes, bias)
 
 
